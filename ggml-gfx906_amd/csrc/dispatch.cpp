@@ -779,6 +779,24 @@ int ggml_mi355x_quantize(const ggml_mi355x_tensor *src, ggml_mi355x_tensor *dst,
     return quantize(view_of(src), view_of(dst), static_cast<hipStream_t>(stream));
 }
 
+static int rope_entry(const ggml_mi355x_tensor *src, const ggml_mi355x_tensor *pos, const ggml_mi355x_tensor *ff,
+                      const ggml_mi355x_tensor *dst, const ggml_mi355x_rope_params *params, bool back, void *stream) {
+    if (!src || !pos || !dst || !params) return GGML_MI355X_EINVAL;
+    TensorView f{};
+    if (ff) f = view_of(ff);
+    return rope(view_of(src), view_of(pos), ff ? &f : nullptr, view_of(dst), *params, back, static_cast<hipStream_t>(stream));
+}
+
+int ggml_mi355x_rope(const ggml_mi355x_tensor *src, const ggml_mi355x_tensor *pos, const ggml_mi355x_tensor *freq_factors,
+                     ggml_mi355x_tensor *dst, const ggml_mi355x_rope_params *params, void *stream) {
+    return rope_entry(src, pos, freq_factors, dst, params, false, stream);
+}
+
+int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const ggml_mi355x_tensor *pos, const ggml_mi355x_tensor *freq_factors,
+                          ggml_mi355x_tensor *dst, const ggml_mi355x_rope_params *params, void *stream) {
+    return rope_entry(src, pos, freq_factors, dst, params, true, stream);
+}
+
 int ggml_mi355x_supports_mul_mat(const ggml_mi355x_tensor *src0, const ggml_mi355x_tensor *src1) {
     if (!src0 || !src1) return 0;
     return is_hot_quant(src0->type) && src1->type == T_F32 && src0->ne[0] % type_blck(src0->type) == 0 &&

@@ -8,6 +8,7 @@
 
 #include <mutex>
 
+#include "../../include/ggml-mi355x.h"
 #include "qmm_args.h"
 
 namespace mi355x {
@@ -141,6 +142,14 @@ struct AttnView {
 };
 constexpr int ATTN_MAX_D = 256, ATTN_MAX_KV = 14336;   // scores of one row live in LDS
 int run_attention(const AttnView &a, hipStream_t st);
+
+// rotary positions and their gradient (rope.hip): src [ne0, heads, tokens, batch] f32 / f16 / bf16,
+// pos i32 [tokens(, batch)], ff f32 [n_dims/2] or nullptr, dst of any of the three types
+typedef ggml_mi355x_rope_params RopeSpec;
+constexpr int ROPE_MAX_DIMS = 512;
+int check_rope(const TensorView &src, const TensorView &pos, const TensorView *ff, const TensorView &dst, const RopeSpec &p);
+int rope(const TensorView &src, const TensorView &pos, const TensorView *ff, const TensorView &dst, const RopeSpec &p, bool back,
+         hipStream_t st);
 
 // quantized mat-vec with the decode-layer fusions (mmvq_fused.hip): layer-norm prologue,
 // bias / GELU / residual epilogue (MmArgs fields); nc columns per launch column group

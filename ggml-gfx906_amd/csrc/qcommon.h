@@ -13,6 +13,7 @@ namespace mi355x {
 // ggml type ids (reference include/ggml.h:372-412)
 enum : int {
     T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q8_0 = 8, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_I32 = 26,
+    T_BF16 = 30,
 };
 
 constexpr int WAVE = 64;

@@ -21,15 +21,25 @@ if os.environ.get("GGML_MI355X_LIB"):
     LIB_PATH = os.environ["GGML_MI355X_LIB"]
 HEADER = os.path.join(os.path.dirname(HERE), "include", "ggml-mi355x.h")
 
-F32, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, I32 = 0, 2, 8, 12, 13, 14, 26
-BLCK = {Q4_0: 32, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, F32: 1, I32: 1}
-TSIZE = {Q4_0: 18, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, F32: 4, I32: 4}
+F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, I32, BF16 = 0, 1, 2, 8, 12, 13, 14, 26, 30
+BLCK = {Q4_0: 32, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, F32: 1, I32: 1, F16: 1, BF16: 1}
+TSIZE = {Q4_0: 18, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, F32: 4, I32: 4, F16: 2, BF16: 2}
 NAMES = {Q4_0: "q4_0", Q8_0: "q8_0", Q4_K: "q4_K", Q5_K: "q5_K", Q6_K: "q6_K"}
 
 
 class MmTensor(C.Structure):
     """ggml_mi355x_tensor (include/ggml-mi355x.h)"""
     _fields_ = [("type", C.c_int32), ("data", C.c_void_p), ("ne", C.c_int64 * 4), ("nb", C.c_size_t * 4)]
+
+
+ROPE_NEIGHBOURS, ROPE_HALVES = 0, 2
+
+
+class RopeSpec(C.Structure):
+    """ggml_mi355x_rope_params"""
+    _fields_ = [("n_dims", C.c_int32), ("mode", C.c_int32), ("n_ctx_orig", C.c_int32), ("freq_base", C.c_float),
+                ("freq_scale", C.c_float), ("ext_factor", C.c_float), ("attn_factor", C.c_float), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float)]
 
 
 class Mi355xError(RuntimeError):
@@ -72,6 +82,8 @@ def lib():
         L.ggml_mi355x_get_rows.argtypes = [P, P, P, C.c_void_p]
         L.ggml_mi355x_quantize.argtypes = [P, P, C.c_void_p]
         L.ggml_mi355x_cpy.argtypes = [P, P, C.c_void_p]
+        for f in (L.ggml_mi355x_rope, L.ggml_mi355x_rope_back):
+            f.argtypes = [P, P, P, P, C.POINTER(RopeSpec), C.c_void_p]
         L.ggml_mi355x_repack_size.argtypes = [P, C.POINTER(C.c_size_t)]
         L.ggml_mi355x_repack.argtypes = [P, C.c_void_p, C.c_size_t, C.c_void_p]
         L.ggml_mi355x_mul_mat_repacked.argtypes = [P, C.c_void_p, P, P, C.c_void_p]
@@ -123,6 +135,21 @@ def tensor(t: int, ptr: int, ne, nb) -> MmTensor:
     return T
 
 
+def from_torch(t) -> MmTensor:
+    """descriptor of a torch tensor of up to 4 dims on the device: its dims innermost first, its strides
+    in bytes (f32, f16, bf16, int32). The tensor must outlive the calls that use the descriptor."""
+    import torch
+    kind = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: I32}.get(t.dtype)
+    if kind is None or t.dim() > 4 or not t.is_cuda:
+        raise Mi355xError(f"from_torch: {t.dtype} of {t.dim()} dims on {t.device} (f32 / f16 / bf16 / int32, <= 4 dims, on a GPU)")
+    e = TSIZE[kind]
+    ne, nb = list(t.shape[::-1]), [s * e for s in t.stride()[::-1]]
+    while len(ne) < 4:
+        nb.append(nb[-1] * ne[-1] if ne else e)
+        ne.append(1)
+    return tensor(kind, t.data_ptr(), ne, nb)
+
+
 def _stream_ptr(stream) -> int | None:
     """hipStream_t for a call: None = torch's current stream; a torch Stream; or a raw handle"""
     if stream is None:
@@ -145,6 +172,27 @@ def get_rows(a: MmTensor, rows: MmTensor, d: MmTensor, stream=None) -> None:
 def quantize(src: MmTensor, dst: MmTensor, stream=None) -> None:
     """dst (Q4_0 / Q8_0) = quantize_row_*_ref(src f32) on the device (GGML_OP_CPY f32 -> q)"""
     _check(lib().ggml_mi355x_quantize(C.byref(src), C.byref(dst), _stream_ptr(stream)), "quantize")
+
+
+def rope_spec(n_dims: int, mode: int = ROPE_NEIGHBOURS, freq_base: float = 10000.0, freq_scale: float = 1.0,
+              n_ctx_orig: int = 0, ext_factor: float = 0.0, attn_factor: float = 1.0, beta_fast: float = 32.0,
+              beta_slow: float = 1.0) -> RopeSpec:
+    return RopeSpec(n_dims, mode, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow)
+
+
+def _ref(t):
+    return None if t is None else C.byref(t)
+
+
+def rope(src: MmTensor, pos: MmTensor, dst: MmTensor, spec: RopeSpec, factors: MmTensor = None, stream=None) -> None:
+    """dst = src with its rows turned by their positions (GGML_OP_ROPE); [ne0, heads, tokens, batch]"""
+    _check(lib().ggml_mi355x_rope(_ref(src), _ref(pos), _ref(factors), _ref(dst), _ref(spec), _stream_ptr(stream)), "rope")
+
+
+def rope_back(src: MmTensor, pos: MmTensor, dst: MmTensor, spec: RopeSpec, factors: MmTensor = None, stream=None) -> None:
+    """dst = the gradient of rope's input for src, the gradient of its result (GGML_OP_ROPE_BACK)"""
+    _check(lib().ggml_mi355x_rope_back(_ref(src), _ref(pos), _ref(factors), _ref(dst), _ref(spec), _stream_ptr(stream)),
+           "rope_back")
 
 
 def repack_size(a: MmTensor) -> int:

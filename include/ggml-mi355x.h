@@ -48,12 +48,14 @@ GGML_MI355X_API struct ggml_backend_reg *ggml_backend_mi355x_reg(void);
 /* ggml type ids used here (reference include/ggml.h:372-412) */
 enum ggml_mi355x_type {
     GGML_MI355X_F32  = 0,
+    GGML_MI355X_F16  = 1,
     GGML_MI355X_Q4_0 = 2,
     GGML_MI355X_Q8_0 = 8,
     GGML_MI355X_Q4_K = 12,
     GGML_MI355X_Q5_K = 13,
     GGML_MI355X_Q6_K = 14,
     GGML_MI355X_I32  = 26,
+    GGML_MI355X_BF16 = 30,
 };
 
 /* error codes (0 = success) */
@@ -124,6 +126,41 @@ GGML_MI355X_API int ggml_mi355x_cpy(const ggml_mi355x_tensor *src, ggml_mi355x_t
  * Same shapes, strided 4-d views with contiguous rows; ne0 a multiple of 32. Replaces
  * ggml_cpy_f32_q4_0_cuda / ggml_cpy_f32_q8_0_cuda (src/ggml-cuda/cpy.cu). */
 GGML_MI355X_API int ggml_mi355x_quantize(const ggml_mi355x_tensor *src, ggml_mi355x_tensor *dst, void *stream);
+
+/* Rotary positions: dst = rope(src) with GGML_OP_ROPE semantics, and the gradient dst = rope_back(src)
+ * (GGML_OP_ROPE_BACK: src is the gradient of rope's result, dst the gradient of its input).
+ *
+ * src, dst: [ne0, heads, tokens, batch] of the same shape, each F32, F16 or BF16 (they may differ: a
+ * key can be turned and rounded straight into a 16-bit cache view), values of a row contiguous,
+ * any strides of whole values above them. dst may be src itself (same type and strides);
+ * otherwise they must not overlap. pos: I32 [tokens] or [tokens, batch], any 32-bit values.
+ * freq_factors: F32 [>= n_dims/2], divisors of the pairs' frequencies, or NULL.
+ *
+ * The first n_dims values of a row turn, the rest are copied. Pairs are neighbours (2i, 2i+1) or the
+ * halves (i, i + n_dims/2); pair i turns by pos * freq_base^(-2i/n_dims) * freq_scale / freq_factors[i],
+ * with YaRN's mix of scaled and unscaled frequencies when ext_factor != 0, and the turned values
+ * are multiplied by attn_factor (* (1 + 0.1 ln(1/freq_scale)) with YaRN). Angles are formed in 64 bits.
+ * EINVAL: other types or modes (multi-section positions), n_dims odd, over 512 or over ne0, shapes
+ * that disagree, freq_base <= 0, or YaRN without n_ctx_orig, freq_base > 1, freq_scale and betas > 0. */
+enum ggml_mi355x_rope_mode {
+    GGML_MI355X_ROPE_NEIGHBOURS = 0,
+    GGML_MI355X_ROPE_HALVES     = 2,
+};
+typedef struct {
+    int32_t n_dims;      /* values of a row that turn, even                                 */
+    int32_t mode;        /* enum ggml_mi355x_rope_mode                                       */
+    int32_t n_ctx_orig;  /* the trained context (YaRN only)                                  */
+    float   freq_base, freq_scale;
+    float   ext_factor;  /* YaRN's mix, 0 = none                                             */
+    float   attn_factor;
+    float   beta_fast, beta_slow;
+} ggml_mi355x_rope_params;
+GGML_MI355X_API int ggml_mi355x_rope(const ggml_mi355x_tensor *src, const ggml_mi355x_tensor *pos,
+                                     const ggml_mi355x_tensor *freq_factors, ggml_mi355x_tensor *dst,
+                                     const ggml_mi355x_rope_params *params, void *stream);
+GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const ggml_mi355x_tensor *pos,
+                                          const ggml_mi355x_tensor *freq_factors, ggml_mi355x_tensor *dst,
+                                          const ggml_mi355x_rope_params *params, void *stream);
 
 /* Repacked weights for the int8 mat-mat tile (the reference's analogue is the CPU
  * backend's repack extra buffer type, src/ggml-cpu/repack.cpp:1967): the quantized codes of src0 as
