@@ -797,6 +797,76 @@ int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const ggml_mi355x_tenso
     return rope_entry(src, pos, freq_factors, dst, params, true, stream);
 }
 
+static int attn_entry(const AttnTensors &t, const ggml_mi355x_attn_params &p, void *work, size_t work_bytes, void *stream) {
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = check_flash_attn(t, p);
+    if (rc != GGML_MI355X_OK) return rc;
+    if (!work) return flash_attn(t, p, st, scratch_for(st));
+    if (work_bytes < flash_attn_work(t) || (uintptr_t)work % 16 != 0) return GGML_MI355X_EINVAL;
+    return flash_attn(t, p, work, st);
+}
+
+// the optional operands of an attention call: views with a place to live
+struct AttnOptional {
+    TensorView v[5];
+    const TensorView *of(int i, const ggml_mi355x_tensor *t) {
+        if (!t) return nullptr;
+        v[i] = view_of(t);
+        return &v[i];
+    }
+};
+
+int ggml_mi355x_flash_attn(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *k, const ggml_mi355x_tensor *v,
+                           const ggml_mi355x_tensor *mask, const ggml_mi355x_tensor *sinks, const ggml_mi355x_tensor *kv_len,
+                           ggml_mi355x_tensor *dst, const ggml_mi355x_attn_params *params, void *work, size_t work_bytes,
+                           void *stream) {
+    if (!q || !k || !v || !dst || !params) return GGML_MI355X_EINVAL;
+    AttnOptional o;
+    AttnTensors t{view_of(q), view_of(k), view_of(v), view_of(dst)};
+    t.mask = o.of(0, mask);
+    t.sinks = o.of(1, sinks);
+    t.len = o.of(2, kv_len);
+    return attn_entry(t, *params, work, work_bytes, stream);
+}
+
+int ggml_mi355x_flash_attn_prefix(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp, const ggml_mi355x_tensor *vp,
+                                  const ggml_mi355x_tensor *k, const ggml_mi355x_tensor *v, const ggml_mi355x_tensor *sinks,
+                                  const ggml_mi355x_tensor *kv_len, ggml_mi355x_tensor *dst,
+                                  const ggml_mi355x_attn_params *params, void *work, size_t work_bytes, void *stream) {
+    if (!q || !kp || !vp || !k || !v || !dst || !params) return GGML_MI355X_EINVAL;
+    AttnOptional o;
+    AttnTensors t{view_of(q), view_of(k), view_of(v), view_of(dst)};
+    t.sinks = o.of(1, sinks);
+    t.len = o.of(2, kv_len);
+    t.kp = o.of(3, kp);
+    t.vp = o.of(4, vp);
+    return attn_entry(t, *params, work, work_bytes, stream);
+}
+
+// (the result's and the values' layouts do not matter here: those of q and k stand in)
+static int attn_work_entry(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp, const ggml_mi355x_tensor *k, size_t *bytes) {
+    if (!q || !k || !bytes) return GGML_MI355X_EINVAL;
+    AttnOptional o;
+    AttnTensors t{view_of(q), view_of(k), view_of(k), view_of(q)};
+    std::swap(t.dst.ne[1], t.dst.ne[2]);
+    std::swap(t.dst.nb[1], t.dst.nb[2]);
+    t.kp = t.vp = o.of(3, kp);
+    const ggml_mi355x_attn_params p{1.0f, 0.0f, 0.0f, 0};
+    const int rc = check_flash_attn(t, p);
+    if (rc != GGML_MI355X_OK) return rc;
+    *bytes = flash_attn_work(t);
+    return GGML_MI355X_OK;
+}
+
+int ggml_mi355x_flash_attn_work_size(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *k, size_t *bytes) {
+    return attn_work_entry(q, nullptr, k, bytes);
+}
+
+int ggml_mi355x_flash_attn_prefix_work_size(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp, const ggml_mi355x_tensor *k,
+                                            size_t *bytes) {
+    return kp ? attn_work_entry(q, kp, k, bytes) : GGML_MI355X_EINVAL;
+}
+
 int ggml_mi355x_supports_mul_mat(const ggml_mi355x_tensor *src0, const ggml_mi355x_tensor *src1) {
     if (!src0 || !src1) return 0;
     return is_hot_quant(src0->type) && src1->type == T_F32 && src0->ne[0] % type_blck(src0->type) == 0 &&

@@ -151,6 +151,18 @@ int check_rope(const TensorView &src, const TensorView &pos, const TensorView *f
 int rope(const TensorView &src, const TensorView &pos, const TensorView *ff, const TensorView &dst, const RopeSpec &p, bool back,
          hipStream_t st);
 
+// attention over a key / value cache (attention.hip); kp / vp: a prefix that every batch shares
+typedef ggml_mi355x_attn_params AttnSpec;
+struct AttnTensors {
+    TensorView q, k, v, dst;
+    const TensorView *mask = nullptr, *sinks = nullptr, *len = nullptr, *kp = nullptr, *vp = nullptr;
+};
+int check_flash_attn(const AttnTensors &t, const AttnSpec &p);
+size_t flash_attn_work(const AttnTensors &t);   // workspace bytes of a call that check_flash_attn accepts
+int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t st);
+// with the workspace taken from `scratch`
+int flash_attn(const AttnTensors &t, const AttnSpec &p, hipStream_t st, Scratch &scratch);
+
 // quantized mat-vec with the decode-layer fusions (mmvq_fused.hip): layer-norm prologue,
 // bias / GELU / residual epilogue (MmArgs fields); nc columns per launch column group
 hipError_t mmvq_fused_launch(int type, const MmArgs &a, int nc, int rpw, hipStream_t st);

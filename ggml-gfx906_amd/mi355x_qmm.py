@@ -42,6 +42,11 @@ class RopeSpec(C.Structure):
                 ("beta_slow", C.c_float)]
 
 
+class AttnSpec(C.Structure):
+    """ggml_mi355x_attn_params"""
+    _fields_ = [("scale", C.c_float), ("max_bias", C.c_float), ("logit_softcap", C.c_float), ("causal", C.c_int32)]
+
+
 class Mi355xError(RuntimeError):
     pass
 
@@ -84,6 +89,11 @@ def lib():
         L.ggml_mi355x_cpy.argtypes = [P, P, C.c_void_p]
         for f in (L.ggml_mi355x_rope, L.ggml_mi355x_rope_back):
             f.argtypes = [P, P, P, P, C.POINTER(RopeSpec), C.c_void_p]
+        A = C.POINTER(AttnSpec)
+        L.ggml_mi355x_flash_attn.argtypes = [P, P, P, P, P, P, P, A, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.ggml_mi355x_flash_attn_work_size.argtypes = [P, P, C.POINTER(C.c_size_t)]
+        L.ggml_mi355x_flash_attn_prefix.argtypes = [P, P, P, P, P, P, P, P, A, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.ggml_mi355x_flash_attn_prefix_work_size.argtypes = [P, P, P, C.POINTER(C.c_size_t)]
         L.ggml_mi355x_repack_size.argtypes = [P, C.POINTER(C.c_size_t)]
         L.ggml_mi355x_repack.argtypes = [P, C.c_void_p, C.c_size_t, C.c_void_p]
         L.ggml_mi355x_mul_mat_repacked.argtypes = [P, C.c_void_p, P, P, C.c_void_p]
@@ -193,6 +203,44 @@ def rope_back(src: MmTensor, pos: MmTensor, dst: MmTensor, spec: RopeSpec, facto
     """dst = the gradient of rope's input for src, the gradient of its result (GGML_OP_ROPE_BACK)"""
     _check(lib().ggml_mi355x_rope_back(_ref(src), _ref(pos), _ref(factors), _ref(dst), _ref(spec), _stream_ptr(stream)),
            "rope_back")
+
+
+def attn_spec(scale: float, max_bias: float = 0.0, logit_softcap: float = 0.0, causal: bool = False) -> AttnSpec:
+    return AttnSpec(scale, max_bias, logit_softcap, 1 if causal else 0)
+
+
+def _work(work):
+    """(address, bytes) of a workspace: a torch tensor, or None for the library's own"""
+    return (None, 0) if work is None else (work.data_ptr(), work.numel() * work.element_size())
+
+
+def flash_attn(q: MmTensor, k: MmTensor, v: MmTensor, dst: MmTensor, spec: AttnSpec, mask: MmTensor = None, sinks: MmTensor = None,
+               kv_len: MmTensor = None, work=None, stream=None) -> None:
+    """dst [D, H, n_q, B] = softmax(scale q k^T + mask) v (GGML_OP_FLASH_ATTN_EXT); q [D, n_q, H, B],
+    k, v [D, n_kv, Hk, Bk]; work: a tensor of flash_attn_work_size bytes"""
+    p, n = _work(work)
+    _check(lib().ggml_mi355x_flash_attn(_ref(q), _ref(k), _ref(v), _ref(mask), _ref(sinks), _ref(kv_len), _ref(dst), _ref(spec),
+                                        p, n, _stream_ptr(stream)), "flash_attn")
+
+
+def flash_attn_work_size(q: MmTensor, k: MmTensor) -> int:
+    n = C.c_size_t(0)
+    _check(lib().ggml_mi355x_flash_attn_work_size(_ref(q), _ref(k), C.byref(n)), "flash_attn_work_size")
+    return n.value
+
+
+def flash_attn_prefix(q: MmTensor, kp: MmTensor, vp: MmTensor, k: MmTensor, v: MmTensor, dst: MmTensor, spec: AttnSpec,
+                      sinks: MmTensor = None, kv_len: MmTensor = None, work=None, stream=None) -> None:
+    """flash_attn of sequences behind a shared prefix kp, vp [D, n_prefix, Hk]; k, v: each one's own cache"""
+    p, n = _work(work)
+    _check(lib().ggml_mi355x_flash_attn_prefix(_ref(q), _ref(kp), _ref(vp), _ref(k), _ref(v), _ref(sinks), _ref(kv_len), _ref(dst),
+                                               _ref(spec), p, n, _stream_ptr(stream)), "flash_attn_prefix")
+
+
+def flash_attn_prefix_work_size(q: MmTensor, kp: MmTensor, k: MmTensor) -> int:
+    n = C.c_size_t(0)
+    _check(lib().ggml_mi355x_flash_attn_prefix_work_size(_ref(q), _ref(kp), _ref(k), C.byref(n)), "flash_attn_prefix_work_size")
+    return n.value
 
 
 def repack_size(a: MmTensor) -> int:

@@ -162,6 +162,57 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
                                           const ggml_mi355x_tensor *freq_factors, ggml_mi355x_tensor *dst,
                                           const ggml_mi355x_rope_params *params, void *stream);
 
+/* Attention over a key / value cache: dst = softmax(scale * q k^T + mask) v, GGML_OP_FLASH_ATTN_EXT's
+ * operands and semantics, computed in one pass (no score matrix in memory).
+ *
+ *   q      [D, n_q, H, B]     F32, F16 or BF16
+ *   k, v   [D, n_kv, Hk, Bk]  F16 or BF16, the same for both; q's type, or F16 with q F32.
+ *                             H a multiple of Hk (query head h reads head h / (H / Hk)), B of Bk
+ *   mask   [>= n_kv, >= n_q, 1 | a divisor of H, 1 | a divisor of B] F16, added to the scaled scores
+ *          (times the head's ALiBi slope if max_bias > 0); -inf hides a key. Or NULL
+ *   sinks  F32 [H]: one more score per head that takes weight and adds no value. Or NULL
+ *   kv_len I32 [B]: keys of each batch in use (read by the kernel; clamped to 0 .. n_kv). Or NULL: n_kv
+ *   dst    [D, H, n_q, B] of q's type (ggml's permuted result)
+ *
+ * causal: the queries are the last n_q of the keys in use, query i sees keys j <= kv_len - n_q + i
+ * (with a mask as well: both hold). Keys that a row does not see take no part in it, whatever their
+ * bytes hold; rows that see no key are zeros. logit_softcap c > 0: scaled scores become
+ * c tanh(score / c) before the mask. F32 queries and weights keep 32-bit accuracy; with F16 / BF16
+ * queries the weights are rounded to that type for the product with v. Results do not depend on
+ * timing: every sum has a fixed order.
+ *
+ * D: a multiple of 8, at most 256. q, k, v, dst: rows contiguous, data and strides multiples of 16
+ * bytes. dst must not overlap the operands. EINVAL for anything else, max_bias > 0 without a mask,
+ * or parameters that are not finite or negative (scale may be negative).
+ *
+ * work: a workspace of ggml_mi355x_flash_attn_work_size() bytes (16-byte aligned), used only until the
+ * call's kernels are done, or NULL: the library keeps one per (device, stream), which can not grow inside
+ * a stream capture (ENOMEM: run the call once before capturing it) and which captured graphs of one
+ * stream share: graphs that may run at the same time need workspaces of their own. */
+typedef struct {
+    float   scale, max_bias, logit_softcap;
+    int32_t causal;  /* 0 or 1 */
+} ggml_mi355x_attn_params;
+GGML_MI355X_API int ggml_mi355x_flash_attn(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *k, const ggml_mi355x_tensor *v,
+                                           const ggml_mi355x_tensor *mask, const ggml_mi355x_tensor *sinks,
+                                           const ggml_mi355x_tensor *kv_len, ggml_mi355x_tensor *dst,
+                                           const ggml_mi355x_attn_params *params, void *work, size_t work_bytes, void *stream);
+/* bytes of workspace for these operands (0: none is needed); it does not depend on kv_len or the mask */
+GGML_MI355X_API int ggml_mi355x_flash_attn_work_size(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *k, size_t *bytes);
+
+/* ggml_mi355x_flash_attn for B sequences that share a prefix: kp, vp [D, n_prefix, Hk, 1] are read once
+ * for all of them, k, v [D, n_kv, Hk, B] are each sequence's own cache behind it, and kv_len I32 [B]
+ * the keys of it in use (NULL: n_kv). Every query sees the whole prefix; with causal = 1 query i sees
+ * its own keys j <= kv_len - n_q + i, with 0 all kv_len. No mask, so max_bias must be 0. */
+GGML_MI355X_API int ggml_mi355x_flash_attn_prefix(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp,
+                                                  const ggml_mi355x_tensor *vp, const ggml_mi355x_tensor *k,
+                                                  const ggml_mi355x_tensor *v, const ggml_mi355x_tensor *sinks,
+                                                  const ggml_mi355x_tensor *kv_len, ggml_mi355x_tensor *dst,
+                                                  const ggml_mi355x_attn_params *params, void *work, size_t work_bytes,
+                                                  void *stream);
+GGML_MI355X_API int ggml_mi355x_flash_attn_prefix_work_size(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp,
+                                                            const ggml_mi355x_tensor *k, size_t *bytes);
+
 /* Repacked weights for the int8 mat-mat tile (the reference's analogue is the CPU
  * backend's repack extra buffer type, src/ggml-cpu/repack.cpp:1967): the quantized codes of src0 as
  * int8 in MFMA-fragment order plus f32 block scales, made once (e.g. at weight upload) so that
