@@ -282,6 +282,63 @@ bool graph_op_of(const struct ggml_tensor *node, GraphOp &g) {
     return true;
 }
 
+// a ROPE / ROPE_BACK node (ggml_rope_ext: op_params n_past, n_dims, mode, n_ctx, n_ctx_orig, then freq_base,
+// freq_scale, ext_factor, attn_factor, beta_fast, beta_slow as f32; src: values, positions[, factors])
+struct RopeNode {
+    TensorView src, pos, ff, dst;
+    bool has_ff;
+    RopeSpec spec;
+};
+bool rope_of(const struct ggml_tensor *node, RopeNode &r) {
+    if ((node->op != GGMLABI_OP_ROPE && node->op != GGMLABI_OP_ROPE_BACK) || !node->src[0] || !node->src[1]) return false;
+    r.src = tv(node->src[0]);
+    r.pos = tv(node->src[1]);
+    r.has_ff = node->src[2] != nullptr;
+    if (r.has_ff) r.ff = tv(node->src[2]);
+    r.dst = tv(node);
+    r.spec.n_dims = node->op_params[1];
+    r.spec.mode = node->op_params[2];
+    r.spec.n_ctx_orig = node->op_params[4];
+    float f[6];
+    std::memcpy(f, &node->op_params[5], sizeof f);
+    r.spec.freq_base = f[0];
+    r.spec.freq_scale = f[1];
+    r.spec.ext_factor = f[2];
+    r.spec.attn_factor = f[3];
+    r.spec.beta_fast = f[4];
+    r.spec.beta_slow = f[5];
+    return true;
+}
+
+// a FLASH_ATTN_EXT node (op_params scale, max_bias, logit_softcap as f32; src: q, k, v[, mask[, sinks]])
+struct AttnNode {
+    AttnTensors t;
+    TensorView mask, sinks;
+    AttnSpec spec;
+};
+bool attn_of(const struct ggml_tensor *node, AttnNode &a) {
+    if (node->op != GGMLABI_OP_FLASH_ATTN_EXT || !node->src[0] || !node->src[1] || !node->src[2]) return false;
+    a.t.q = tv(node->src[0]);
+    a.t.k = tv(node->src[1]);
+    a.t.v = tv(node->src[2]);
+    a.t.dst = tv(node);
+    if (node->src[3]) {
+        a.mask = tv(node->src[3]);
+        a.t.mask = &a.mask;
+    }
+    if (node->src[4]) {
+        a.sinks = tv(node->src[4]);
+        a.t.sinks = &a.sinks;
+    }
+    float f[3];
+    std::memcpy(f, node->op_params, sizeof f);
+    a.spec.scale = f[0];
+    a.spec.max_bias = f[1];
+    a.spec.logit_softcap = f[2];
+    a.spec.causal = 0;
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------
 // buffer
 // ------------------------------------------------------------------------------------------
@@ -1759,6 +1816,8 @@ enum ggml_status run_nodes(BackendCtx *c, struct ggml_cgraph *g, bool quiet, boo
         if (is_empty(node) || is_view_op(node->op) || plan.skip[i]) continue;
         int rc = GGML_MI355X_OK;
         GraphOp gop;
+        RopeNode rn;
+        AttnNode an;
         int fused = 0;
         auto at = plan.attn.find(i);
         auto lr = plan.layers.find(i);
@@ -1789,6 +1848,10 @@ enum ggml_status run_nodes(BackendCtx *c, struct ggml_cgraph *g, bool quiet, boo
             rc = cpy(tv(node->src[0]), tv(node), c->stream);   // for CPY node is the view of src[1]
         } else if (graph_op_of(node, gop)) {
             rc = run_graph_op(gop, c->stream);
+        } else if (rope_of(node, rn)) {
+            rc = rope(rn.src, rn.pos, rn.has_ff ? &rn.ff : nullptr, rn.dst, rn.spec, node->op == GGMLABI_OP_ROPE_BACK, c->stream);
+        } else if (attn_of(node, an)) {
+            rc = flash_attn(an.t, an.spec, c->stream, c->scratch);
         } else {
             fprintf(stderr, "[ggml-mi355x] unsupported op %d in graph (node %s)\n", node->op, node->name);
             return GGML_STATUS_FAILED;
@@ -2088,6 +2151,16 @@ bool dv_supports_op(ggml_backend_dev_t d, const struct ggml_tensor *op) {
         case GGMLABI_OP_DUP:
             if (is_quant_copy(op)) return check_cpy(tv(op->src[0]), tv(op)) == GGML_MI355X_OK;
             break;
+        // rotary positions: neighbouring and half pairs (multi-section positions stay on the CPU backend)
+        case GGMLABI_OP_ROPE:
+        case GGMLABI_OP_ROPE_BACK: {
+            RopeNode r;
+            return rope_of(op, r) && check_rope(r.src, r.pos, r.has_ff ? &r.ff : nullptr, r.dst, r.spec) == GGML_MI355X_OK;
+        }
+        case GGMLABI_OP_FLASH_ATTN_EXT: {
+            AttnNode a;
+            return attn_of(op, a) && check_flash_attn(a.t, a.spec) == GGML_MI355X_OK;
+        }
         default:
             break;
     }

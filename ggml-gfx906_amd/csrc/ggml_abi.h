@@ -47,6 +47,9 @@ enum {
     GGMLABI_OP_DIAG_MASK_INF = 43,
     GGMLABI_OP_DIAG_MASK_ZERO = 44,
     GGMLABI_OP_SOFT_MAX = 45,
+    GGMLABI_OP_ROPE = 47,
+    GGMLABI_OP_ROPE_BACK = 48,
+    GGMLABI_OP_FLASH_ATTN_EXT = 67,
     GGMLABI_OP_UNARY = 78,
 };
 

@@ -45,6 +45,9 @@ int main() {
     E(GGMLABI_OP_DIAG_MASK_INF, GGML_OP_DIAG_MASK_INF)
     E(GGMLABI_OP_DIAG_MASK_ZERO, GGML_OP_DIAG_MASK_ZERO)
     E(GGMLABI_OP_SOFT_MAX, GGML_OP_SOFT_MAX)
+    E(GGMLABI_OP_ROPE, GGML_OP_ROPE)
+    E(GGMLABI_OP_ROPE_BACK, GGML_OP_ROPE_BACK)
+    E(GGMLABI_OP_FLASH_ATTN_EXT, GGML_OP_FLASH_ATTN_EXT)
     E(GGMLABI_OP_UNARY, GGML_OP_UNARY)
     E(GGMLABI_UNARY_OP_GELU, GGML_UNARY_OP_GELU)
     E(GGMLABI_OP_MUL_MAT, GGML_OP_MUL_MAT)
