@@ -171,8 +171,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) char lds_char;
-typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef const __attribute__((address_space(3))) char *lds_const;
 
 constexpr float BIAS = 8.0f, LAZY = 7.0f;
 constexpr int MAX_SLOTS = 256;   // partial results of a row
@@ -197,9 +196,19 @@ struct AttnPart {
     int rows, row_tiles;       // of each
 };
 
-// 4 rows of 16-byte pieces by LDS DMA
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, char *lds, uint32_t voff, uint32_t soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, voff, soff, 0, 0);
+// 16 bytes per lane from base + voff + soff into LDS at dst + 16 * lane (dst, soff wave-uniform). Written out
+// because the compiler, which can not tell the stages apart, makes every LDS read wait for each DMA that it
+// knows of; the kernel waits itself. No result registers; the address registers are read at issue. The
+// nops are the wait states from a scalar's write by a vector instruction and from m0's to their use.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 buffer_at(const char *p) {   // a raw buffer of 2 GiB
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    return i32x4{(int)__builtin_amdgcn_readfirstlane((uint32_t)at), (int)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32) & 0xffff), 0x7fffffff, 0x00020000};
+}
+__device__ __forceinline__ void dma16(i32x4 r, const char *dst, uint32_t voff, uint32_t soff) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_const)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(at), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
 
 template <typename TK, typename TQ, int DP, bool BY_ROWS, bool PREFIX>
@@ -436,7 +445,7 @@ template <int DP>
 __device__ __forceinline__ uint32_t piece_off(int place, int swz, int D) { return (uint32_t)(min(place ^ swz, D / 8 - 1) * 16); }
 
 template <typename TK, typename TQ, int DP, bool BY_ROWS, bool PREFIX>
-__global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)) void attn_tile_kernel(const AttnArgs a, const AttnPart p) {
+__global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64), (BY_ROWS && DP <= 128 ? 2 : 1)) void attn_tile_kernel(const AttnArgs a, const AttnPart p) {
     using T = AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT;
@@ -474,6 +483,49 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
     j_begin = __builtin_amdgcn_readfirstlane(j_begin);
     j_end = __builtin_amdgcn_readfirstlane(j_end);
     const int seen = min(j_end, !PREFIX && a.causal ? n - a.n_q + i + 1 : n);
+
+    const bool masked = !PREFIX && a.mask != nullptr;
+    const char *mrow = nullptr;
+    float slope = 0.0f;
+    if (masked) {
+        mrow = a.mask + i * a.m_i + (head % a.m_nh) * a.m_h + (b % a.m_nb) * a.m_b;
+        slope = slope_of(a, head) * LOG2E;
+    }
+
+    const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + (int64_t)(pb / a.kv_b) * a.k_b;
+    const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + (int64_t)(pb / a.kv_b) * a.v_b;
+    const int64_t k_j = PREFIX ? a.kp_j : a.k_j, v_j = PREFIX ? a.vp_j : a.v_j;
+
+    // the tile at key j into stage `st` of this wave's (BY_ROWS: the workgroup's) LDS
+    const int ltid = BY_ROWS ? tid : lane, lrow = ltid / CPR, place = ltid % CPR;
+    char *stage0 = lds + (BY_ROWS ? 0 : wave * 4 * BYTES);
+    const uint32_t k_row = (uint32_t)lrow * (uint32_t)k_j, v_row = (uint32_t)lrow * (uint32_t)v_j;
+    auto load = [&](int j, int st) {
+        char *kd = stage0 + st * 2 * BYTES + (BY_ROWS ? wave * 1024 : 0), *vd = kd + BYTES;
+        const i32x4 kr = buffer_at(kb + j * k_j), vr = buffer_at(vb + j * v_j);
+        const int last = j_end - 1 - j;
+        if (last >= KT - 1) {
+#pragma unroll
+            for (int u = 0; u < ROUNDS; ++u) {
+                const int r = u * RPI + lrow;
+                dma16(kr, kd + u * T::LOADERS * 16, k_row + piece_off<DP>(place, swz_k<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)k_j);
+                dma16(vr, vd + u * T::LOADERS * 16, v_row + piece_off<DP>(place, swz_v<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)v_j);
+            }
+        } else {   // rows behind the keys: the last key again
+#pragma unroll
+            for (int u = 0; u < ROUNDS; ++u) {
+                const int r = u * RPI + lrow;
+                const uint32_t rr = (uint32_t)min(r, last);
+                dma16(kr, kd + u * T::LOADERS * 16, rr * (uint32_t)k_j + piece_off<DP>(place, swz_k<DP>(r), a.D), 0);
+                dma16(vr, vd + u * T::LOADERS * 16, rr * (uint32_t)v_j + piece_off<DP>(place, swz_v<DP>(r), a.D), 0);
+            }
+        }
+    };
+
+    // the first tile's DMA, then the queries, then one wait for both: the compiler, which knows of the
+    // latter only, would otherwise wait inside the loop, and there for the tile ahead too
+    const int j0 = BY_ROWS ? j_begin : j_begin + wave * 32;
+    if (j0 < j_end) load(j0, 0);
 
     // queries: lane (row, h) holds values 16 t + 8 h .. + 7 of its row
     x8 qf[NT], ql[SPLIT ? NT : 1];
@@ -533,47 +585,31 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
         }
     }
     c = fmaxf(c, 0x1p-126f);
-    const char *mrow = nullptr;
-    float slope = 0.0f;
-    if (!PREFIX && a.mask) {
-        mrow = a.mask + i * a.m_i + (head % a.m_nh) * a.m_h + (b % a.m_nb) * a.m_b;
-        slope = slope_of(a, head) * LOG2E;
-    }
-
-    const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + (int64_t)(pb / a.kv_b) * a.k_b;
-    const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + (int64_t)(pb / a.kv_b) * a.v_b;
-    const int64_t k_j = PREFIX ? a.kp_j : a.k_j, v_j = PREFIX ? a.vp_j : a.v_j;
-
-    // the tile at key j into stage `st` of this wave's (BY_ROWS: the workgroup's) LDS
-    const int ltid = BY_ROWS ? tid : lane, lrow = ltid / CPR, place = ltid % CPR;
-    char *stage0 = lds + (BY_ROWS ? 0 : wave * 4 * BYTES);
-    const uint32_t k_row = (uint32_t)lrow * (uint32_t)k_j, v_row = (uint32_t)lrow * (uint32_t)v_j;
-    auto load = [&](int j, int st) {
-        char *kd = stage0 + st * 2 * BYTES + (BY_ROWS ? wave * 1024 : 0), *vd = kd + BYTES;
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(kb) + j * k_j, 0, 0x7fffffff, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(vb) + j * v_j, 0, 0x7fffffff, 0x00020000);
-        const int last = j_end - 1 - j;   // (rows behind the keys: the last key again)
-#pragma unroll
-        for (int u = 0; u < ROUNDS; ++u) {
-            const int r = u * RPI + lrow;
-            const uint32_t ko = piece_off<DP>(place, swz_k<DP>(r), a.D), vo = piece_off<DP>(place, swz_v<DP>(r), a.D);
-            if (last >= KT - 1) {
-                dma16(kr, kd + u * T::LOADERS * 16, k_row + ko, (uint32_t)(u * RPI) * (uint32_t)k_j);
-                dma16(vr, vd + u * T::LOADERS * 16, v_row + vo, (uint32_t)(u * RPI) * (uint32_t)v_j);
-            } else {
-                const uint32_t rr = (uint32_t)min(r, last);
-                dma16(kr, kd + u * T::LOADERS * 16, rr * (uint32_t)k_j + ko, 0);
-                dma16(vr, vd + u * T::LOADERS * 16, rr * (uint32_t)v_j + vo, 0);
-            }
-        }
-    };
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
 
     f32x16 o[NB];
 #pragma unroll
     for (int d = 0; d < NB; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.0f;   // (l: of the lane's own keys)
 
-    auto compute = [&](int j, int st) {
+    // the mask's values at the tile's keys, in the order of the scores
+    auto fetch = [&](int j, f16x4 (&w)[KT / 8]) {
+        const int left = seen - j - 4 * h;
+#pragma unroll
+        for (int r = 0; r < KT / 8; ++r) {
+            const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 8 * r + 4 * h;
+            w[r] = f16x4{};
+            if (a.m_vec && 8 * r + 4 <= left) {
+                w[r] = *reinterpret_cast<const f16x4 *>(mp);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * r + e < left) w[r][e] = mp[e];
+            }
+        }
+    };
+
+    auto compute = [&](int j, int st, const f16x4 (&w)[KT / 8]) {
         const char *kt = stage0 + st * 2 * BYTES, *vt = kt + BYTES;
         f32x16 s[KT / 32];
         const int krow = lane & 31, ksw = swz_k<DP>(krow);
@@ -591,34 +627,19 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
         // of log 2
         const int left = seen - j - 4 * h;
         float f = c;
-        if (capped || mrow) {
+        if (capped || masked) {
             f = 1.0f;
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const int j0 = 32 * u + 8 * r4;
-                    f16x4 add{};
-                    if (mrow) {
-                        const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + j0 + 4 * h;
-                        if (a.m_vec && j0 + 4 <= left) {
-                            add = *reinterpret_cast<const f16x4 *>(mp);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (j0 + e < left) add[e] = mp[e];
-                        }
+                for (int r = 0; r < 16; ++r) {
+                    float x = s[u][r];
+                    x = capped ? cap2 * tanhf(x * c_cap) : x * c;
+                    if (masked) {
+                        const float add = (float)w[4 * u + r / 4][r % 4];
+                        x = add == -INFINITY ? -INFINITY : fmaf(slope, add, x);
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = s[u][4 * r4 + e];
-                        x = capped ? cap2 * tanhf(x * c_cap) : x * c;
-                        if (mrow) {
-                            const float w = (float)add[e];
-                            x = w == -INFINITY ? -INFINITY : fmaf(slope, w, x);
-                        }
-                        s[u][4 * r4 + e] = x;
-                    }
+                    s[u][r] = x;
                 }
         }
         if (__any(seen - j < KT)) {
@@ -679,23 +700,35 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
     if constexpr (BY_ROWS) {
         // (a later row sees no fewer keys)
         const int seen_most = row0 < p.rows ? __builtin_amdgcn_readlane(seen, 31) : 0;
-        if (j_begin < j_end) load(j_begin, 0);
+        f16x4 w[KT / 8], ahead[KT / 8];
+        if (masked && j_begin < j_end) fetch(j_begin, ahead);
         int st = 0;
         for (int j = j_begin; j < j_end; j += KT, st ^= 1) {
             // this wave's share of the tile has come; behind the barrier everyone's has, and the other stage is read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (j + KT < j_end) load(j + KT, st ^ 1);
-            if (j < seen_most) compute(j, st);
+            if (masked) {   // (moved here, so that the compiler's wait for them comes before the next DMA)
+#pragma unroll
+                for (int r = 0; r < KT / 8; ++r) {
+                    w[r] = ahead[r];
+                    asm volatile("" : "+v"(w[r]));
+                }
+            }
+            if (j + KT < j_end) {
+                load(j + KT, st ^ 1);
+                if (masked) fetch(j + KT, ahead);
+            }
+            if (j < seen_most) compute(j, st, w);
         }
     } else {
         constexpr int STEP = T::WAVES * 32;
-        int j = j_begin + wave * 32, st = 0;
-        if (j < j_end) load(j, 0);
+        int j = j0, st = 0;
+        f16x4 w[KT / 8];
         if (j + STEP < j_end) load(j + STEP, 1);
         for (; j < j_end; j += STEP, st ^= 1) {
+            if (masked) fetch(j, w);
             if (j + STEP < j_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * ROUNDS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            compute(j, st);
+            compute(j, st, w);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage is read
             if (j + 2 * STEP < j_end) load(j + 2 * STEP, st);
         }
