@@ -36,11 +36,17 @@ struct RopeArgs {
     double turns[ROPE_MAX_DIMS / 2];  // f_i / 2pi
 };
 
-__device__ __forceinline__ float ldf(const char *p, int i, float) { return reinterpret_cast<const float *>(p)[i]; }
-__device__ __forceinline__ float ldf(const char *p, int i, _Float16) { return (float)reinterpret_cast<const _Float16 *>(p)[i]; }
-__device__ __forceinline__ float ldf(const char *p, int i, __bf16) { return (float)reinterpret_cast<const __bf16 *>(p)[i]; }
+// cosine and sine of pair p at position `pos`, times the factor
+__device__ __forceinline__ void turn(const RopeArgs &a, int p, double pos, float &cs, float &sn) {
+    double t = pos * a.turns[p];
+    if (a.factors) t /= (double)a.factors[p];
+    t -= rint(t);
+    sincospif(2.0f * (float)t, &sn, &cs);
+    cs *= a.size;
+    sn *= a.size * a.way;
+}
 
-// one thread per pair, then one per copied value
+// any layout: one thread per pair, then one per copied value
 template <typename TS, typename TD>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     const int half = a.n_dims / 2, units = half + (a.ne0 - a.n_dims);
@@ -49,24 +55,71 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
         const int64_t row = u / units;
         const int p = (int)(u % units);
         const int64_t h = row % a.ne1, t = row / a.ne1 % a.ne2, b = row / a.ne1 / a.ne2;
-        const char *s = a.src + h * a.s_h + t * a.s_t + b * a.s_b;
+        const TS *s = reinterpret_cast<const TS *>(a.src + h * a.s_h + t * a.s_t + b * a.s_b);
         TD *d = reinterpret_cast<TD *>(a.dst + h * a.d_h + t * a.d_t + b * a.d_b);
         if (p >= half) {
-            const int i = p + half;
-            d[i] = (TD)ldf(s, i, TS{});
+            d[p + half] = (TD)(float)s[p + half];
             continue;
         }
-        double turn = (double)a.pos[b * a.pos_b + t] * a.turns[p];
-        if (a.factors) turn /= (double)a.factors[p];
-        turn -= rint(turn);
-        float sn, cs;
-        sincospif(2.0f * (float)turn, &sn, &cs);
-        cs *= a.size;
-        sn *= a.size * a.way;
+        float cs, sn;
+        turn(a, p, (double)a.pos[b * a.pos_b + t], cs, sn);
         const int ia = a.halves ? p : 2 * p, ib = a.halves ? p + half : 2 * p + 1;
-        const float x = ldf(s, ia, TS{}), y = ldf(s, ib, TS{});
+        const float x = (float)s[ia], y = (float)s[ib];
         d[ia] = (TD)(x * cs - y * sn);
         d[ib] = (TD)(x * sn + y * cs);
+    }
+}
+
+// Rows of whole groups of 8 values at 16-byte (f32) / 8-byte places: a thread turns the same 4 pairs of
+// HEADS heads of one token, so their sines are formed once, and all its loads are issued before them.
+// Bound by memory: 4096 tokens x 32 heads x 128 f32 values, 134 MB in 24.4 us, 5.5 TB/s; 8192 x 8 x 128 f32
+// into f16 12.4 us, 4.1 TB/s; a token's 32 heads 3.5 us, the launch.
+template <typename T> struct RopeVec { typedef T x4 __attribute__((ext_vector_type(4))); };
+
+template <typename TS, typename TD, bool HALVES, int HEADS>
+__global__ __launch_bounds__(256) void rope_vec_kernel(const RopeArgs a) {
+    typedef typename RopeVec<TS>::x4 S4;
+    typedef typename RopeVec<TD>::x4 D4;
+    const uint32_t units = (uint32_t)a.ne0 / 8, at = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t t = at / units, u = at % units;
+    if (t >= (uint32_t)a.ne2) return;
+    const int h0 = blockIdx.y * HEADS, b = blockIdx.z;
+    const bool turns = u < (uint32_t)a.n_dims / 8;
+    // the two groups of four values
+    const int i0 = HALVES && turns ? 4 * u : 8 * u, i1 = HALVES && turns ? 4 * u + a.n_dims / 2 : 8 * u + 4;
+    const char *s = a.src + (int64_t)t * a.s_t + b * a.s_b;
+    char *d = a.dst + (int64_t)t * a.d_t + b * a.d_b;
+    S4 x[HEADS], y[HEADS];
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+        const TS *r = reinterpret_cast<const TS *>(s + min(h0 + k, a.ne1 - 1) * a.s_h);
+        x[k] = *reinterpret_cast<const S4 *>(r + i0);
+        y[k] = *reinterpret_cast<const S4 *>(r + i1);
+    }
+    float cs[4] = {}, sn[4] = {};
+    if (turns) {
+        const double pos = (double)a.pos[b * a.pos_b + t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) turn(a, 4 * u + e, pos, cs[e], sn[e]);
+    }
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+        if (h0 + k >= a.ne1) break;
+        TD *r = reinterpret_cast<TD *>(d + (h0 + k) * a.d_h);
+        float v[8], w[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = (float)x[k][e];
+            v[4 + e] = (float)y[k][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int ia = HALVES ? e : 2 * e, ib = HALVES ? e + 4 : 2 * e + 1;
+            w[ia] = turns ? v[ia] * cs[e] - v[ib] * sn[e] : v[ia];
+            w[ib] = turns ? v[ia] * sn[e] + v[ib] * cs[e] : v[ib];
+        }
+        *reinterpret_cast<D4 *>(r + i0) = D4{(TD)w[0], (TD)w[1], (TD)w[2], (TD)w[3]};
+        *reinterpret_cast<D4 *>(r + i1) = D4{(TD)w[4], (TD)w[5], (TD)w[6], (TD)w[7]};
     }
 }
 
@@ -104,11 +157,40 @@ void rope_turns(const RopeSpec &p, double *turns, float *size) {
 bool rope_type(int t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
 int rope_bytes(int t) { return t == T_F32 ? 4 : 2; }
 
+template <typename TS, typename TD>
+void rope_launch(const RopeArgs &g, int64_t batches, hipStream_t st) {
+    auto fits = [](const void *p, int64_t h, int64_t t, int64_t b, int to) { return (uintptr_t)p % to == 0 && h % to == 0 && t % to == 0 && b % to == 0; };
+    const int64_t units = g.ne0 / 8, threads = units * g.ne2;
+    const bool vec = g.ne0 % 8 == 0 && g.n_dims % 8 == 0 && fits(g.src, g.s_h, g.s_t, g.s_b, 4 * sizeof(TS)) &&
+                     fits(g.dst, g.d_h, g.d_t, g.d_b, 4 * sizeof(TD)) && threads < (1LL << 31) && batches <= 65535 && g.ne1 <= 65535;
+    if (!vec) {
+        const int64_t n = g.rows * (g.n_dims / 2 + g.ne0 - g.n_dims);
+        hipLaunchKernelGGL((rope_kernel<TS, TD>), dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, st, g);
+        return;
+    }
+    const unsigned blocks = (unsigned)((threads + 255) / 256);
+    // One head a thread until that makes 4 waves for each SIMD of the 256 CUs; from there on the sines cost
+    // more than further waves hide, and a thread takes 8 heads (4 where there are fewer): 4096 x 32 x 128 f32
+    // 42.9 us with a pair a thread, 30.9 / 25.4 / 24.4 / 23.4 with 2 / 4 / 8 / 16 heads; 4 x 1000 x 20 x 80
+    // bf16 12.9 with one, 9.8 / 8.6 / 8.0 / 9.9.
+    const int heads = threads * g.ne1 * batches < 4LL * 4 * 256 * 64 || g.ne1 == 1 ? 1 : g.ne1 < 8 ? 4 : 8;
+    const dim3 grid(blocks, (unsigned)((g.ne1 + heads - 1) / heads), (unsigned)batches);
+#define ROPE_CASE(N)                                                                                             \
+    if (heads == N) {                                                                                            \
+        if (g.halves) hipLaunchKernelGGL((rope_vec_kernel<TS, TD, true, N>), grid, dim3(256), 0, st, g);          \
+        else hipLaunchKernelGGL((rope_vec_kernel<TS, TD, false, N>), grid, dim3(256), 0, st, g);                  \
+    }
+    ROPE_CASE(1)
+    ROPE_CASE(4)
+    ROPE_CASE(8)
+#undef ROPE_CASE
+}
+
 template <typename TS>
-void rope_pick(int td, dim3 grid, const RopeArgs &g, hipStream_t st) {
-    if (td == T_F32) hipLaunchKernelGGL((rope_kernel<TS, float>), grid, dim3(256), 0, st, g);
-    else if (td == T_F16) hipLaunchKernelGGL((rope_kernel<TS, _Float16>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((rope_kernel<TS, __bf16>), grid, dim3(256), 0, st, g);
+void rope_pick(int td, const RopeArgs &g, int64_t batches, hipStream_t st) {
+    if (td == T_F32) rope_launch<TS, float>(g, batches, st);
+    else if (td == T_F16) rope_launch<TS, _Float16>(g, batches, st);
+    else rope_launch<TS, __bf16>(g, batches, st);
 }
 
 }  // namespace
@@ -153,17 +235,19 @@ int rope(const TensorView &s, const TensorView &pos, const TensorView *ff, const
     g.factors = ff ? static_cast<const float *>(ff->data) : nullptr;
     g.s_h = (int64_t)s.nb[1]; g.s_t = (int64_t)s.nb[2]; g.s_b = (int64_t)s.nb[3];
     g.d_h = (int64_t)d.nb[1]; g.d_t = (int64_t)d.nb[2]; g.d_b = (int64_t)d.nb[3];
+    // (a dim of one index has any stride: none, so that it is aligned)
+    if (s.ne[1] == 1) g.s_h = g.d_h = 0;
+    if (s.ne[2] == 1) g.s_t = g.d_t = 0;
+    if (s.ne[3] == 1) g.s_b = g.d_b = 0;
     g.pos_b = pos.ne[1] > 1 ? (int64_t)pos.nb[1] / 4 : 0;
     g.ne0 = (int)s.ne[0]; g.ne1 = (int)s.ne[1]; g.ne2 = (int)s.ne[2];
     g.n_dims = p.n_dims;
     g.halves = p.mode == GGML_MI355X_ROPE_HALVES;
     g.way = back ? -1.0f : 1.0f;
     rope_turns(p, g.turns, &g.size);
-    const int64_t units = g.rows * (g.n_dims / 2 + g.ne0 - g.n_dims);
-    const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 1 << 20));
-    if (s.type == T_F32) rope_pick<float>(d.type, grid, g, st);
-    else if (s.type == T_F16) rope_pick<_Float16>(d.type, grid, g, st);
-    else rope_pick<__bf16>(d.type, grid, g, st);
+    if (s.type == T_F32) rope_pick<float>(d.type, g, s.ne[3], st);
+    else if (s.type == T_F16) rope_pick<_Float16>(d.type, g, s.ne[3], st);
+    else rope_pick<__bf16>(d.type, g, s.ne[3], st);
     return hipGetLastError() == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
 }
 
