@@ -1,0 +1,177 @@
+// attention.cpp — checks, plan and launch of attention over a key / value cache and behind a shared prefix
+// (kernels: attention_impl.h)
+#include "../../include/ggml-mi355x.h"
+#include "attention.h"
+#include "dispatch.h"
+#include "qcommon.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mi355x {
+
+namespace {
+
+int elem(int t) { return t == T_F32 ? 4 : 2; }
+
+// data and the strides of the dims that have more than one index: multiples of `to`
+bool aligned_to(const TensorView &t, size_t to) {
+    if ((uintptr_t)t.data % to != 0) return false;
+    for (int i = 1; i < 4; ++i)
+        if (t.ne[i] > 1 && t.nb[i] % to != 0) return false;
+    return true;
+}
+
+// 16-byte aligned rows of contiguous values (an empty tensor has no rows to look at)
+bool rows_fit(const TensorView &t) {
+    if (t.ne[0] == 0 || t.ne[1] == 0 || t.ne[2] == 0 || t.ne[3] == 0) return true;
+    return (int64_t)t.nb[0] == elem(t.type) && aligned_to(t, 16);
+}
+
+bool dims_fit(const TensorView &t) {
+    for (int i = 0; i < 4; ++i)
+        if (t.ne[i] < 0 || t.ne[i] > (1 << 30)) return false;
+    return true;
+}
+
+}  // namespace
+
+// shapes, types and layouts of flash_attn (kp / vp: nullptr) and flash_attn_prefix
+static int check_attn(const AttnTensors &t, const AttnSpec &p) {
+    const TensorView &q = t.q, &k = t.k, &v = t.v, &d = t.dst;
+    if (k.type != v.type || !(k.type == T_F16 || k.type == T_BF16)) return GGML_MI355X_EINVAL;
+    if (q.type != d.type || !(q.type == k.type || (q.type == T_F32 && k.type == T_F16))) return GGML_MI355X_EINVAL;
+    for (const TensorView *x : {&q, &k, &v, &d})
+        if (!dims_fit(*x) || !rows_fit(*x)) return GGML_MI355X_EINVAL;
+    const int64_t D = q.ne[0], n_q = q.ne[1], H = q.ne[2], B = q.ne[3];
+    if (D < 8 || D > ATTN_MAX_D || D % 8 != 0 || k.ne[0] != D || v.ne[0] != D) return GGML_MI355X_EINVAL;
+    for (int i = 1; i < 4; ++i)
+        if (k.ne[i] != v.ne[i]) return GGML_MI355X_EINVAL;
+    if (k.ne[2] <= 0 || H % k.ne[2] != 0 || k.ne[3] <= 0 || B % k.ne[3] != 0) return GGML_MI355X_EINVAL;
+    // (32-bit row and workgroup counts, with room for 512 splits or row tiles)
+    if (H > 65535 || B > 65535 || n_q > (1 << 24) || (double)H * B * std::max<int64_t>(1, n_q) > (double)(1 << 28)) return GGML_MI355X_EINVAL;
+    if (d.ne[0] != D || d.ne[1] != H || d.ne[2] != n_q || d.ne[3] != B) return GGML_MI355X_EINVAL;
+    for (int i = 1; i < 4; ++i)
+        if (d.ne[i] > 1 && d.nb[i] == 0) return GGML_MI355X_EINVAL;   // two rows in one place
+    if (t.kp) {
+        const TensorView &kp = *t.kp, &vp = *t.vp;
+        if (kp.type != k.type || vp.type != k.type || t.mask) return GGML_MI355X_EINVAL;
+        for (const TensorView *x : {&kp, &vp})
+            if (!dims_fit(*x) || !rows_fit(*x) || x->ne[0] != D || x->ne[2] != k.ne[2] || x->ne[3] != 1 || x->ne[1] != kp.ne[1])
+                return GGML_MI355X_EINVAL;
+        if (k.ne[3] != B) return GGML_MI355X_EINVAL;   // every sequence has its own cache
+    }
+    if (t.mask) {
+        const TensorView &m = *t.mask;
+        if (m.type != T_F16 || !dims_fit(m) || m.nb[0] != 2 || !aligned_to(m, 2) || m.ne[0] < k.ne[1] || m.ne[1] < n_q) return GGML_MI355X_EINVAL;
+        if (m.ne[2] <= 0 || m.ne[3] <= 0 || H % m.ne[2] != 0 || B % m.ne[3] != 0) return GGML_MI355X_EINVAL;
+    }
+    if (t.sinks && (t.sinks->type != T_F32 || t.sinks->ne[0] < H || t.sinks->nb[0] != 4 || (uintptr_t)t.sinks->data % 4 != 0)) return GGML_MI355X_EINVAL;
+    if (t.len) {
+        const TensorView &l = *t.len;
+        if (l.type != T_I32 || l.ne[0] != B || (B > 1 && l.nb[0] % 4 != 0) || (uintptr_t)l.data % 4 != 0) return GGML_MI355X_EINVAL;
+    }
+    if (!std::isfinite(p.scale) || !(p.max_bias >= 0.0f) || !std::isfinite(p.max_bias) || !(p.logit_softcap >= 0.0f) ||
+        !std::isfinite(p.logit_softcap) || !(p.causal == 0 || p.causal == 1))
+        return GGML_MI355X_EINVAL;
+    if (p.max_bias > 0.0f && !t.mask) return GGML_MI355X_EINVAL;   // slopes multiply a mask
+    return GGML_MI355X_OK;
+}
+
+int check_flash_attn(const AttnTensors &t, const AttnSpec &p) { return check_attn(t, p); }
+
+static AttnPlan plan_attn(const AttnTensors &t) {
+    AttnPlan p{};
+    const int64_t n_q = t.q.ne[1], H = t.q.ne[2], B = t.q.ne[3], Hk = t.k.ne[2], G = H / Hk;
+    // the tile kernel's offsets inside a tile are 32-bit: positions up to 16 MiB apart
+    p.tiled = true;
+    for (const TensorView *x : {&t.k, &t.v, t.kp, t.vp})
+        if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
+    if (!p.tiled) return p;
+    auto pick = [](int64_t rows, int64_t problems, int64_t keys, bool &by_rows, int &tiles, int &splits) {
+        by_rows = rows > 32;
+        tiles = (int)((rows + (by_rows ? 127 : 31)) / (by_rows ? 128 : 32));
+        const int64_t groups = std::max<int64_t>(1, problems * tiles);
+        splits = (int)std::max<int64_t>(1, std::min({(512 + groups - 1) / groups, (keys + 127) / 128, (int64_t)ATTN_MAX_SLOTS / 2}));
+        if (groups >= 256) splits = 1;
+    };
+    pick(n_q * G, B * Hk, t.k.ne[1], p.own_rows, p.own_tiles, p.own_splits);
+    p.slots = p.own_splits;
+    if (t.kp) {
+        pick(B * n_q * G, Hk, t.kp->ne[1], p.pre_rows, p.pre_tiles, p.pre_splits);
+        p.slots += p.pre_splits;
+    }
+    return p;
+}
+
+size_t flash_attn_work(const AttnTensors &t) {
+    const AttnPlan p = plan_attn(t);
+    return p.slots > 1 ? (size_t)t.q.ne[1] * t.q.ne[2] * t.q.ne[3] * p.slots * (t.q.ne[0] + 2) * sizeof(float) : 0;
+}
+
+static bool has_data(const AttnTensors &t) {
+    return t.q.data && t.dst.data && (t.k.ne[1] == 0 || (t.k.data && t.v.data)) && (!t.kp || t.kp->ne[1] == 0 || (t.kp->data && t.vp->data)) &&
+           (!t.mask || t.mask->data) && (!t.sinks || t.sinks->data) && (!t.len || t.len->data);
+}
+
+int flash_attn(const AttnTensors &t, const AttnSpec &p, hipStream_t st, Scratch &scratch) {
+    const int rc = check_attn(t, p);
+    if (rc != GGML_MI355X_OK) return rc;
+    const size_t bytes = flash_attn_work(t);
+    if (bytes == 0 || !has_data(t)) return flash_attn(t, p, nullptr, st);
+    std::lock_guard<std::mutex> hold(scratch.mu);   // until the kernels that use it are queued
+    void *work = scratch.get(bytes, st);
+    return work ? flash_attn(t, p, work, st) : GGML_MI355X_ENOMEM;
+}
+
+int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t st) {
+    const int rc = check_attn(t, p);
+    if (rc != GGML_MI355X_OK) return rc;
+    const TensorView &q = t.q, &k = t.k, &v = t.v, &d = t.dst;
+    if (q.ne[1] == 0 || q.ne[2] == 0 || q.ne[3] == 0) return GGML_MI355X_OK;
+    if (!has_data(t)) return GGML_MI355X_EINVAL;
+    AttnArgs a{};
+    a.q = static_cast<const char *>(q.data);
+    a.q_i = (int64_t)q.nb[1]; a.q_h = (int64_t)q.nb[2]; a.q_b = (int64_t)q.nb[3];
+    a.k = static_cast<const char *>(k.data);
+    a.k_j = (int64_t)k.nb[1]; a.k_h = (int64_t)k.nb[2]; a.k_b = (int64_t)k.nb[3];
+    a.v = static_cast<const char *>(v.data);
+    a.v_j = (int64_t)v.nb[1]; a.v_h = (int64_t)v.nb[2]; a.v_b = (int64_t)v.nb[3];
+    if (t.kp) {
+        a.kp = static_cast<const char *>(t.kp->data);
+        a.kp_j = (int64_t)t.kp->nb[1]; a.kp_h = (int64_t)t.kp->nb[2];
+        a.vp = static_cast<const char *>(t.vp->data);
+        a.vp_j = (int64_t)t.vp->nb[1]; a.vp_h = (int64_t)t.vp->nb[2];
+        a.n_prefix = (int)t.kp->ne[1];
+    }
+    if (t.mask) {
+        a.mask = static_cast<const char *>(t.mask->data);
+        a.m_i = (int64_t)t.mask->nb[1]; a.m_h = (int64_t)t.mask->nb[2]; a.m_b = (int64_t)t.mask->nb[3];
+        a.m_nh = (int)t.mask->ne[2]; a.m_nb = (int)t.mask->ne[3];
+        a.m_vec = aligned_to(*t.mask, 8);
+    }
+    if (t.sinks) a.sinks = static_cast<const float *>(t.sinks->data);
+    if (t.len) {
+        a.len = static_cast<const char *>(t.len->data);
+        a.len_b = (int64_t)t.len->nb[0];
+    }
+    a.o = static_cast<char *>(d.data);
+    a.o_h = (int64_t)d.nb[1]; a.o_i = (int64_t)d.nb[2]; a.o_b = (int64_t)d.nb[3];
+    a.D = (int)q.ne[0]; a.n_q = (int)q.ne[1]; a.n_kv = (int)k.ne[1];
+    a.H = (int)q.ne[2]; a.Hk = (int)k.ne[2]; a.B = (int)q.ne[3]; a.kv_b = (int)(q.ne[3] / k.ne[3]);
+    a.causal = p.causal;
+    a.scale = p.scale;
+    a.cap = p.logit_softcap;
+    if (p.max_bias > 0.0f) {
+        a.bias_heads = 1 << (int)std::floor(std::log2((double)a.H));
+        a.m0 = std::pow(2.0f, -p.max_bias / a.bias_heads);
+        a.m1 = std::pow(2.0f, -p.max_bias / 2.0f / a.bias_heads);
+    }
+    const AttnPlan pl = plan_attn(t);
+    const hipError_t e = q.type == T_F32   ? attn_launch_f16_f32(a, pl, work, st)
+                         : q.type == T_F16 ? attn_launch_f16(a, pl, work, st)
+                                           : attn_launch_bf16(a, pl, work, st);
+    return e == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
+}
+
+}  // namespace mi355x

@@ -1,0 +1,10 @@
+// attention_f16.hip — the attention kernels (attention_impl.h) for f16 cache and activations
+#include "attention_impl.h"
+
+namespace mi355x {
+
+hipError_t attn_launch_f16(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
+    return launch_attn_any<_Float16, _Float16>(a, pl, work, st);
+}
+
+}  // namespace mi355x

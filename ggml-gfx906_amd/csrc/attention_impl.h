@@ -1,4 +1,4 @@
-// attention.hip — softmax(scale * Q K^T + mask) V over a key / value cache (GGML_OP_FLASH_ATTN_EXT),
+// attention_impl.h — softmax(scale * Q K^T + mask) V over a key / value cache (GGML_OP_FLASH_ATTN_EXT),
 // and the same for sequences that share one long prefix.
 //
 // Per (batch b, head h, query i), with hk = h / (H / Hk) the shared key / value head:
@@ -7,37 +7,16 @@
 // over the keys j < len_b that the mask leaves (not -inf) and, when causal, j <= len_b - n_q + i.
 // A row that sees nothing is zeros. A key that a row does not see takes no part in it, whatever its
 // bytes hold: caches are not cleared, and a NaN times a weight of 0 would be NaN.
-#include "../../include/ggml-mi355x.h"
-#include "dispatch.h"
-#include "qcommon.h"
+#pragma once
 
-#include <algorithm>
-#include <cmath>
+#include "attention.h"
+#include "qcommon.h"
 
 namespace mi355x {
 
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
-
-struct AttnArgs {
-    const char *q; int64_t q_i, q_h, q_b;
-    const char *k; int64_t k_j, k_h, k_b;
-    const char *v; int64_t v_j, v_h, v_b;
-    const char *kp; int64_t kp_j, kp_h;              // the shared prefix, or n_prefix = 0
-    const char *vp; int64_t vp_j, vp_h;
-    const char *mask; int64_t m_i, m_h, m_b;         // f16, or nullptr
-    int m_nh, m_nb;                                  // its head and batch planes
-    bool m_vec;                                      // rows of 8-byte aligned groups of four
-    const float *sinks;
-    const char *len; int64_t len_b;                  // i32 [batch], or nullptr: n_kv
-    char *o; int64_t o_i, o_h, o_b;
-    int D, n_q, n_kv, n_prefix, H, Hk, B, kv_b;      // kv_b: batches that share one cache
-    int causal;
-    float scale, cap;                                // cap = 0: none
-    int bias_heads;                                  // slopes: 0 = none, else the power of two of heads
-    float m0, m1;
-};
 
 __device__ __forceinline__ float wave_add(float v) {
 #pragma unroll
@@ -174,7 +153,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(3))) char *lds_const;
 
 constexpr float BIAS = 8.0f, LAZY = 7.0f;
-constexpr int MAX_SLOTS = 256;   // partial results of a row
 
 template <typename T> struct Vec;
 template <> struct Vec<_Float16> { typedef f16x8 x8; };
@@ -187,19 +165,20 @@ __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __b
 template <int DP> __device__ __forceinline__ int swz_k(int r) { return DP == 64 ? (r >> 1) & 7 : r & 15; }
 template <int DP> __device__ __forceinline__ int swz_v(int r) { return DP == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; }
 
-// which keys and rows a launch works on
+// which keys and rows some of a launch's workgroups work on
 struct AttnPart {
     float *part_o, *part_ml;   // partial results, or nullptr: the call's result
-    int slot0, n_split;        // this launch's splits among
+    int slot0, n_split;        // these splits among
     int slots;                 // all partial results of a row
     int n_bh;                  // (batch,) key / value head problems
     int rows, row_tiles;       // of each
+    int blocks;
 };
 
 // 16 bytes per lane from base + voff + soff into LDS at dst + 16 * lane (dst, soff wave-uniform). Written out
 // because the compiler, which can not tell the stages apart, makes every LDS read wait for each DMA that it
-// knows of; the kernel waits itself. No result registers; the address registers are read at issue. The
-// nops are the wait states from a scalar's write by a vector instruction and from m0's to their use.
+// knows of; the kernel waits itself. No result registers; the address registers are read at issue; m0 is
+// a reserved register, which the compiler sets right before an own use (these kernels have none). The nops are the wait states from a scalar's write by a vector instruction and from m0's to their use.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4 buffer_at(const char *p) {   // a raw buffer of 2 GiB
     const uint64_t at = (uint64_t)(uintptr_t)p;
@@ -211,17 +190,19 @@ __device__ __forceinline__ void dma16(i32x4 r, const char *dst, uint32_t voff, u
                  :: "s"(at), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
 
-template <typename TK, typename TQ, int DP, bool BY_ROWS, bool PREFIX>
+template <typename TK, typename TQ, int DP, bool BY_ROWS>
 struct AttnTile {
     static constexpr bool SPLIT = sizeof(TQ) == 4;
     static constexpr int KT = BY_ROWS && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int CPR = DP / 8;                          // 16-byte pieces of a row
-    static constexpr int WAVES = !BY_ROWS && DP == 256 ? 2 : 4; // (two stages of every wave's tiles fit the 160 KB)
     static constexpr int LOADERS = BY_ROWS ? 256 : 64;          // threads that load a tile together
     static constexpr int RPI = LOADERS / CPR;                   // rows of one DMA round
     static constexpr int ROUNDS = KT / RPI;
     static constexpr int BYTES = KT * DP * 2;                   // of a tile of keys, and of values
-    static constexpr int LDS = (BY_ROWS ? 1 : WAVES) * 4 * BYTES;   // keys and values, two stages
+    // BY_ROWS: two stages of keys and values; else one of each per wave, whose 32 rows also fit it as f32,
+    // and those rows' maxima and sums
+    static constexpr int STRETCH = BY_ROWS ? 4 * BYTES : 2 * BYTES + 256;
+    static constexpr int LDS = (BY_ROWS ? 1 : 4) * STRETCH;
     typedef typename Vec<TK>::x8 x8;
 };
 
@@ -341,12 +322,12 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
     }
 }
 
-// 32 rows that `waves` waves hold parts of, each in its stretch of LDS (values [row][DP], then the
-// maxima and the sums): THREADS / 32 threads a row
-template <typename TK, typename TQ, int DP, int WAVES, bool PREFIX>
+// 32 rows that the four waves hold parts of, each in its stretch of LDS (values [row][DP], then the
+// maxima and the sums): 8 threads a row
+template <typename TK, typename TQ, int DP, bool PREFIX>
 __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p, const char *lds, int stretch, int tops, int row0, int bh,
                                            int split, int j_begin, int j_end) {
-    constexpr int TPR = WAVES * 2, N = DP / TPR;
+    constexpr int WAVES = 4, TPR = 8, N = DP / TPR;
     const int r = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N, row = row0 + r;
     const bool ok = row < p.rows;
     float m = -INFINITY, l = 0.0f, f[WAVES];
@@ -403,57 +384,69 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p,
     }
 }
 
-// the splits' partial results of a row, in their order: one wave a row, groups of DP / 4 lanes take
-// every other split
+// the splits' partial results of a row: a workgroup a row, groups of DP / 4 threads take every GROUPS-th
+// split and are joined in their order
 template <typename TQ, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a, const AttnPart p) {
-    __shared__ float weight[4][MAX_SLOTS];
-    constexpr int LPR = DP / 4, GROUPS = 64 / LPR;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t rr = (int64_t)blockIdx.x * 4 + wave;
+    constexpr int LPR = DP / 4, GROUPS = 256 / LPR;
+    __shared__ float weight[ATTN_MAX_SLOTS];
+    __shared__ f32x4 part[GROUPS][LPR];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t rr = blockIdx.x;
     const int G = a.H / a.Hk, per = a.n_q * G;
-    if (rr >= (int64_t)a.B * a.Hk * per) return;
     const int r = (int)(rr % per), hk = (int)(rr / per % a.Hk), b = (int)(rr / per / a.Hk), i = r / G, head = hk * G + r % G;
+    const int d = tid % LPR * 4, grp = tid / LPR;
+    const float *po = p.part_o + rr * p.slots * a.D + d;
+    // (at most ATTN_MAX_SLOTS / GROUPS values a thread: the first ones are on their way while the weights form)
+    f32x4 x0{}, x1{};
+    if (d < a.D) {
+        if (grp < p.slots) x0 = *reinterpret_cast<const f32x4 *>(po + (int64_t)grp * a.D);
+        if (grp + GROUPS < p.slots) x1 = *reinterpret_cast<const f32x4 *>(po + (int64_t)(grp + GROUPS) * a.D);
+    }
     const float *ml = p.part_ml + 2 * rr * p.slots;
-    float m = -INFINITY;
+    float m = -INFINITY;   // (every wave looks at all of them)
     for (int s = lane; s < p.slots; s += 64) m = fmaxf(m, ml[2 * s]);
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
     float l = 0.0f;
     for (int s = lane; s < p.slots; s += 64) {
         const float f = m == -INFINITY ? 1.0f : exp2f(ml[2 * s] - m);
-        weight[wave][s] = f;
+        if (tid < 64) weight[s] = f;
         l += ml[2 * s + 1] * f;
     }
     l = wave_add(l);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the wave's own weights)
-    const int d = lane % LPR * 4, grp = lane / LPR;
+    __syncthreads();
     f32x4 x{};
-    if (d < a.D)
-        for (int s = grp; s < p.slots; s += GROUPS) x += *reinterpret_cast<const f32x4 *>(p.part_o + (rr * p.slots + s) * a.D + d) * weight[wave][s];
-#pragma unroll
-    for (int s = LPR; s < 64; s <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], s, 64);
+    if (grp < p.slots) x += x0 * weight[grp];
+    if (grp + GROUPS < p.slots) x += x1 * weight[grp + GROUPS];
+    if (d < a.D) {
+#pragma unroll 4
+        for (int s = grp + 2 * GROUPS; s < p.slots; s += GROUPS) x += *reinterpret_cast<const f32x4 *>(po + (int64_t)s * a.D) * weight[s];
+    }
+    part[grp][tid % LPR] = x;
+    __syncthreads();
     if (grp != 0 || d >= a.D) return;
+    const int most = min(GROUPS, p.slots);
+    for (int g = 1; g < most; ++g) x += part[g][tid];
     TQ *out = reinterpret_cast<TQ *>(a.o + i * a.o_i + head * a.o_h + b * a.o_b);
     store4<TQ>(out + d, x * finish(a, head, m, l));
 }
 
 // one round of pieces: LDS place `slot` (row slot / CPR, place slot % CPR) takes row `row` of the tensor's tile
-template <int DP>
 __device__ __forceinline__ uint32_t piece_off(int place, int swz, int D) { return (uint32_t)(min(place ^ swz, D / 8 - 1) * 16); }
 
-template <typename TK, typename TQ, int DP, bool BY_ROWS, bool PREFIX>
-__global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64), (BY_ROWS && DP <= 128 ? 2 : 1)) void attn_tile_kernel(const AttnArgs a, const AttnPart p) {
-    using T = AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>;
+// a batch's own keys without a mask or a cap, with either; behind a shared prefix; the prefix (the last two
+// have no mask, and may have a cap)
+enum AttnKind { OWN, OWN_GENERAL, OWN_BEHIND, PREFIX_KEYS };
+
+template <typename TK, typename TQ, int DP, bool BY_ROWS, AttnKind KIND>
+__device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p, char *lds, int id) {
+    using T = AttnTile<TK, TQ, DP, BY_ROWS>;
     typedef typename T::x8 x8;
-    constexpr bool SPLIT = T::SPLIT;
+    constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
     constexpr int KT = T::KT, CPR = T::CPR, RPI = T::RPI, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DP / 16, NB = DP / 32;
-    __shared__ __align__(16) char lds[T::LDS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     // problem, row tile (the last ones first: with a causal rule they see the most keys), split of the keys
-    int id = blockIdx.x;
     const int bh = id % p.n_bh;
     id /= p.n_bh;
     const int split = id % p.n_split, tile = p.row_tiles - 1 - id / p.n_split;
@@ -484,7 +477,7 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
     j_end = __builtin_amdgcn_readfirstlane(j_end);
     const int seen = min(j_end, !PREFIX && a.causal ? n - a.n_q + i + 1 : n);
 
-    const bool masked = !PREFIX && a.mask != nullptr;
+    const bool masked = KIND == OWN_GENERAL && a.mask != nullptr;
     const char *mrow = nullptr;
     float slope = 0.0f;
     if (masked) {
@@ -496,36 +489,34 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
     const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + (int64_t)(pb / a.kv_b) * a.v_b;
     const int64_t k_j = PREFIX ? a.kp_j : a.k_j, v_j = PREFIX ? a.vp_j : a.v_j;
 
-    // the tile at key j into stage `st` of this wave's (BY_ROWS: the workgroup's) LDS
+    // the tile at key j into `dst`, this wave's (BY_ROWS: the workgroup's) LDS
     const int ltid = BY_ROWS ? tid : lane, lrow = ltid / CPR, place = ltid % CPR;
-    char *stage0 = lds + (BY_ROWS ? 0 : wave * 4 * BYTES);
-    const uint32_t k_row = (uint32_t)lrow * (uint32_t)k_j, v_row = (uint32_t)lrow * (uint32_t)v_j;
-    auto load = [&](int j, int st) {
-        char *kd = stage0 + st * 2 * BYTES + (BY_ROWS ? wave * 1024 : 0), *vd = kd + BYTES;
-        const i32x4 kr = buffer_at(kb + j * k_j), vr = buffer_at(vb + j * v_j);
+    char *stage0 = lds + (BY_ROWS ? 0 : wave * T::STRETCH);
+    auto load = [&](const char *base, int64_t stride, int j, char *dst, auto swz) {
+        char *to = dst + (BY_ROWS ? wave * 1024 : 0);
+        const i32x4 buf = buffer_at(base + j * stride);
+        const uint32_t step = (uint32_t)stride;
         const int last = j_end - 1 - j;
         if (last >= KT - 1) {
 #pragma unroll
-            for (int u = 0; u < ROUNDS; ++u) {
-                const int r = u * RPI + lrow;
-                dma16(kr, kd + u * T::LOADERS * 16, k_row + piece_off<DP>(place, swz_k<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)k_j);
-                dma16(vr, vd + u * T::LOADERS * 16, v_row + piece_off<DP>(place, swz_v<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)v_j);
-            }
+            for (int u = 0; u < ROUNDS; ++u)
+                dma16(buf, to + u * T::LOADERS * 16, lrow * step + piece_off(place, swz(u * RPI + lrow), a.D), (uint32_t)(u * RPI) * step);
         } else {   // rows behind the keys: the last key again
 #pragma unroll
-            for (int u = 0; u < ROUNDS; ++u) {
-                const int r = u * RPI + lrow;
-                const uint32_t rr = (uint32_t)min(r, last);
-                dma16(kr, kd + u * T::LOADERS * 16, rr * (uint32_t)k_j + piece_off<DP>(place, swz_k<DP>(r), a.D), 0);
-                dma16(vr, vd + u * T::LOADERS * 16, rr * (uint32_t)v_j + piece_off<DP>(place, swz_v<DP>(r), a.D), 0);
-            }
+            for (int u = 0; u < ROUNDS; ++u)
+                dma16(buf, to + u * T::LOADERS * 16, (uint32_t)min(u * RPI + lrow, last) * step + piece_off(place, swz(u * RPI + lrow), a.D), 0);
         }
     };
+    auto load_k = [&](int j, char *dst) { load(kb, k_j, j, dst, [](int r) { return swz_k<DP>(r); }); };
+    auto load_v = [&](int j, char *dst) { load(vb, v_j, j, dst, [](int r) { return swz_v<DP>(r); }); };
 
     // the first tile's DMA, then the queries, then one wait for both: the compiler, which knows of the
     // latter only, would otherwise wait inside the loop, and there for the tile ahead too
     const int j0 = BY_ROWS ? j_begin : j_begin + wave * 32;
-    if (j0 < j_end) load(j0, 0);
+    if (j0 < j_end) {
+        load_k(j0, stage0);
+        load_v(j0, stage0 + BYTES);
+    }
 
     // queries: lane (row, h) holds values 16 t + 8 h .. + 7 of its row
     x8 qf[NT], ql[SPLIT ? NT : 1];
@@ -571,7 +562,7 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
             }
         }
     }
-    const bool capped = a.cap != 0.0f;
+    const bool capped = KIND != OWN && a.cap != 0.0f;
     const float c_cap = capped ? c / a.cap : 0.0f, cap2 = a.cap * LOG2E;
     c *= LOG2E;
     // the maximum is taken of the bare products, so their factor must be above 0: its sign goes into
@@ -594,24 +585,21 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
 
     // the mask's values at the tile's keys, in the order of the scores
     auto fetch = [&](int j, f16x4 (&w)[KT / 8]) {
-        const int left = seen - j - 4 * h;
+        const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 4 * h;
+        if (a.m_vec && __all(seen - j >= KT)) {
 #pragma unroll
-        for (int r = 0; r < KT / 8; ++r) {
-            const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 8 * r + 4 * h;
-            w[r] = f16x4{};
-            if (a.m_vec && 8 * r + 4 <= left) {
-                w[r] = *reinterpret_cast<const f16x4 *>(mp);
-            } else {
+            for (int r = 0; r < KT / 8; ++r) w[r] = *reinterpret_cast<const f16x4 *>(mp + 8 * r);
+        } else {
+            const int left = seen - j - 4 * h;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (8 * r + e < left) w[r][e] = mp[e];
-            }
+            for (int r = 0; r < KT / 8; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[r][e] = 8 * r + e < left ? mp[8 * r + e] : (_Float16)0.0f;
         }
     };
 
-    auto compute = [&](int j, int st, const f16x4 (&w)[KT / 8]) {
-        const char *kt = stage0 + st * 2 * BYTES, *vt = kt + BYTES;
-        f32x16 s[KT / 32];
+    f32x16 s[KT / 32];
+    auto products = [&](const char *kt) {
         const int krow = lane & 31, ksw = swz_k<DP>(krow);
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
@@ -623,8 +611,10 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
                 if constexpr (SPLIT) s[u] = mma(kf, ql[t], s[u]);
             }
         }
-        // s[u][r] is the product of key j + 32 u + 8 (r / 4) + 4 h + r % 4; f times it is the score in units
-        // of log 2
+    };
+    // the weights of the tile's keys from their products: s[u][r] belongs to key j + 32 u + 8 (r / 4) + 4 h +
+    // r % 4, f times it is the score in units of log 2
+    auto weights = [&](int j, const f16x4 (&w)[KT / 8]) {
         const int left = seen - j - 4 * h;
         float f = c;
         if (capped || masked) {
@@ -673,6 +663,8 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
                 sum += s[u][r];
             }
         l += sum;
+    };
+    auto values = [&](const char *vt) {
         // O^T += V^T P^T, 16 keys a step: the lane's weights 8 (t % 2) .. + 7 of block t / 2
         const int vi = lane & 15, vrow = 4 * h + (vi >> 2), vch = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1), vsw = swz_v<DP>(vrow);
 #pragma unroll
@@ -702,8 +694,8 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
         const int seen_most = row0 < p.rows ? __builtin_amdgcn_readlane(seen, 31) : 0;
         f16x4 w[KT / 8], ahead[KT / 8];
         if (masked && j_begin < j_end) fetch(j_begin, ahead);
-        int st = 0;
-        for (int j = j_begin; j < j_end; j += KT, st ^= 1) {
+        char *now = stage0, *next = stage0 + 2 * BYTES;
+        for (int j = j_begin; j < j_end; j += KT) {
             // this wave's share of the tile has come; behind the barrier everyone's has, and the other stage is read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (masked) {   // (moved here, so that the compiler's wait for them comes before the next DMA)
@@ -714,33 +706,57 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
                 }
             }
             if (j + KT < j_end) {
-                load(j + KT, st ^ 1);
+                load_k(j + KT, next);
+                load_v(j + KT, next + BYTES);
                 if (masked) fetch(j + KT, ahead);
             }
-            if (j < seen_most) compute(j, st, w);
+            if (j < seen_most) {
+                products(now);
+                weights(j, w);
+                values(now + BYTES);
+            }
+            char *t = now;
+            now = next;
+            next = t;
         }
     } else {
-        constexpr int STEP = T::WAVES * 32;
-        int j = j0, st = 0;
-        f16x4 w[KT / 8];
-        if (j + STEP < j_end) load(j + STEP, 1);
-        for (; j < j_end; j += STEP, st ^= 1) {
-            if (masked) fetch(j, w);
-            if (j + STEP < j_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * ROUNDS) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            compute(j, st, w);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage is read
-            if (j + 2 * STEP < j_end) load(j + 2 * STEP, st);
+        // a tile's keys are refilled once their products are formed, its values behind those, so that either
+        // is on its way while the other is worked on
+        constexpr int STEP = 4 * 32;
+        f16x4 w[KT / 8], ahead[KT / 8];
+        if (masked && j0 < j_end) fetch(j0, ahead);
+        for (int j = j0; j < j_end; j += STEP) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory");   // the keys
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < KT / 8; ++r) {
+                    w[r] = ahead[r];
+                    asm volatile("" : "+v"(w[r]));
+                }
+                if (j + STEP < j_end) fetch(j + STEP, ahead);
+            }
+            products(stage0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (j + STEP < j_end) {
+                load_k(j + STEP, stage0);
+                weights(j, w);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory");   // the values
+            } else {
+                weights(j, w);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            values(stage0 + BYTES);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (j + STEP < j_end) load_v(j + STEP, stage0 + BYTES);
         }
     }
     l += swap32_f(l);
     const float me = m - BIAS;   // (-inf: no key)
 
     if constexpr (!BY_ROWS) {
-        // join the waves: each leaves its rows in its own stages, wave w then joins values w * DP/4 ..
+        // join the waves: each leaves its rows in its own stretch
         asm volatile("" ::: "memory");
-        float *po = reinterpret_cast<float *>(lds + wave * 4 * BYTES);   // [row][DP], DP * 128 bytes = 2 BYTES
-        float *pm = reinterpret_cast<float *>(lds + wave * 4 * BYTES + 2 * BYTES);
+        float *po = reinterpret_cast<float *>(stage0), *pm = reinterpret_cast<float *>(stage0 + 2 * BYTES);
 #pragma unroll
         for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -753,151 +769,69 @@ __global__ __launch_bounds__((AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64)
             pm[32 + lane] = l;
         }
         __syncthreads();
-        join_waves<TK, TQ, DP, T::WAVES, PREFIX>(a, p, lds, 4 * BYTES, 2 * BYTES, row0, bh, split, j_begin, j_end);
+        join_waves<TK, TQ, DP, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
     } else {
         store_rows<TK, TQ, DP, PREFIX>(a, p, o, me, l, row, row_ok, bh, split, j_begin, j_end);
     }
 }
 
-int elem(int t) { return t == T_F32 ? 4 : 2; }
-
-// data and the strides of the dims that have more than one index: multiples of `to`
-bool aligned_to(const TensorView &t, size_t to) {
-    if ((uintptr_t)t.data % to != 0) return false;
-    for (int i = 1; i < 4; ++i)
-        if (t.ne[i] > 1 && t.nb[i] % to != 0) return false;
-    return true;
-}
-
-// 16-byte aligned rows of contiguous values (an empty tensor has no rows to look at)
-bool rows_fit(const TensorView &t) {
-    if (t.ne[0] == 0 || t.ne[1] == 0 || t.ne[2] == 0 || t.ne[3] == 0) return true;
-    return (int64_t)t.nb[0] == elem(t.type) && aligned_to(t, 16);
-}
-
-bool dims_fit(const TensorView &t) {
-    for (int i = 0; i < 4; ++i)
-        if (t.ne[i] < 0 || t.ne[i] > (1 << 30)) return false;
-    return true;
-}
-
-}  // namespace
-
-// shapes, types and layouts of flash_attn (kp / vp: nullptr) and flash_attn_prefix
-static int check_attn(const AttnTensors &t, const AttnSpec &p) {
-    const TensorView &q = t.q, &k = t.k, &v = t.v, &d = t.dst;
-    if (k.type != v.type || !(k.type == T_F16 || k.type == T_BF16)) return GGML_MI355X_EINVAL;
-    if (q.type != d.type || !(q.type == k.type || (q.type == T_F32 && k.type == T_F16))) return GGML_MI355X_EINVAL;
-    for (const TensorView *x : {&q, &k, &v, &d})
-        if (!dims_fit(*x) || !rows_fit(*x)) return GGML_MI355X_EINVAL;
-    const int64_t D = q.ne[0], n_q = q.ne[1], H = q.ne[2], B = q.ne[3];
-    if (D < 8 || D > ATTN_MAX_D || D % 8 != 0 || k.ne[0] != D || v.ne[0] != D) return GGML_MI355X_EINVAL;
-    for (int i = 1; i < 4; ++i)
-        if (k.ne[i] != v.ne[i]) return GGML_MI355X_EINVAL;
-    if (k.ne[2] <= 0 || H % k.ne[2] != 0 || k.ne[3] <= 0 || B % k.ne[3] != 0) return GGML_MI355X_EINVAL;
-    if (H > 65535 || B > 65535 || n_q > (1 << 24)) return GGML_MI355X_EINVAL;
-    if (d.ne[0] != D || d.ne[1] != H || d.ne[2] != n_q || d.ne[3] != B) return GGML_MI355X_EINVAL;
-    for (int i = 1; i < 4; ++i)
-        if (d.ne[i] > 1 && d.nb[i] == 0) return GGML_MI355X_EINVAL;   // two rows in one place
-    if (t.kp) {
-        const TensorView &kp = *t.kp, &vp = *t.vp;
-        if (kp.type != k.type || vp.type != k.type || t.mask) return GGML_MI355X_EINVAL;
-        for (const TensorView *x : {&kp, &vp})
-            if (!dims_fit(*x) || !rows_fit(*x) || x->ne[0] != D || x->ne[2] != k.ne[2] || x->ne[3] != 1 || x->ne[1] != kp.ne[1])
-                return GGML_MI355X_EINVAL;
-        if (k.ne[3] != B) return GGML_MI355X_EINVAL;   // every sequence has its own cache
+// One launch: the workgroups of a shared prefix (PRE: 0 none, 1 split keys, 2 row tiles), which are bound
+// by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs
+template <typename TK, typename TQ, int DP, int PRE, bool OWN_ROWS, bool GENERAL>
+__global__ __launch_bounds__(256, DP == 256 || (DP == 128 && GENERAL && sizeof(TQ) == 4) ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre,
+                                                                                                    const AttnPart own) {
+    constexpr int L0 = AttnTile<TK, TQ, DP, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DP, PRE == 2>::LDS;
+    __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
+    if constexpr (PRE != 0) {
+        if ((int)blockIdx.x < pre.blocks) {
+            attn_tiles<TK, TQ, DP, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
+            return;
+        }
     }
-    if (t.mask) {
-        const TensorView &m = *t.mask;
-        if (m.type != T_F16 || !dims_fit(m) || m.nb[0] != 2 || !aligned_to(m, 2) || m.ne[0] < k.ne[1] || m.ne[1] < n_q) return GGML_MI355X_EINVAL;
-        if (m.ne[2] <= 0 || m.ne[3] <= 0 || H % m.ne[2] != 0 || B % m.ne[3] != 0) return GGML_MI355X_EINVAL;
-    }
-    if (t.sinks && (t.sinks->type != T_F32 || t.sinks->ne[0] < H || t.sinks->nb[0] != 4 || (uintptr_t)t.sinks->data % 4 != 0)) return GGML_MI355X_EINVAL;
-    if (t.len) {
-        const TensorView &l = *t.len;
-        if (l.type != T_I32 || l.ne[0] != B || (B > 1 && l.nb[0] % 4 != 0) || (uintptr_t)l.data % 4 != 0) return GGML_MI355X_EINVAL;
-    }
-    if (!std::isfinite(p.scale) || !(p.max_bias >= 0.0f) || !std::isfinite(p.max_bias) || !(p.logit_softcap >= 0.0f) ||
-        !std::isfinite(p.logit_softcap) || !(p.causal == 0 || p.causal == 1))
-        return GGML_MI355X_EINVAL;
-    if (p.max_bias > 0.0f && !t.mask) return GGML_MI355X_EINVAL;   // slopes multiply a mask
-    return GGML_MI355X_OK;
-}
-
-int check_flash_attn(const AttnTensors &t, const AttnSpec &p) { return check_attn(t, p); }
-
-// what a call launches, by its shapes alone
-struct AttnPlan {
-    bool tiled;                              // else attn_rows_kernel
-    bool own_rows, pre_rows;                 // row tiles of 128 (4 waves of 32), or 32 rows with split keys
-    int own_tiles, own_splits, pre_tiles, pre_splits, slots;
-};
-
-static AttnPlan plan_attn(const AttnTensors &t) {
-    AttnPlan p{};
-    const int64_t n_q = t.q.ne[1], H = t.q.ne[2], B = t.q.ne[3], Hk = t.k.ne[2], G = H / Hk;
-    // the tile kernel's offsets inside a tile are 32-bit: positions up to 16 MiB apart
-    p.tiled = true;
-    for (const TensorView *x : {&t.k, &t.v, t.kp, t.vp})
-        if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
-    if (!p.tiled) return p;
-    auto pick = [](int64_t rows, int64_t problems, int64_t keys, bool &by_rows, int &tiles, int &splits) {
-        by_rows = rows > 32;
-        tiles = (int)((rows + (by_rows ? 127 : 31)) / (by_rows ? 128 : 32));
-        const int64_t groups = std::max<int64_t>(1, problems * tiles);
-        splits = (int)std::max<int64_t>(1, std::min({(512 + groups - 1) / groups, (keys + 127) / 128, (int64_t)MAX_SLOTS / 2}));
-        if (groups >= 256) splits = 1;
-    };
-    pick(n_q * G, B * Hk, t.k.ne[1], p.own_rows, p.own_tiles, p.own_splits);
-    p.slots = p.own_splits;
-    if (t.kp) {
-        pick(B * n_q * G, Hk, t.kp->ne[1], p.pre_rows, p.pre_tiles, p.pre_splits);
-        p.slots += p.pre_splits;
-    }
-    return p;
-}
-
-size_t flash_attn_work(const AttnTensors &t) {
-    const AttnPlan p = plan_attn(t);
-    return p.slots > 1 ? (size_t)t.q.ne[1] * t.q.ne[2] * t.q.ne[3] * p.slots * (t.q.ne[0] + 2) * sizeof(float) : 0;
-}
-
-template <typename TK, typename TQ, int DP, bool BY_ROWS, bool PREFIX>
-static void launch_tiles(const AttnArgs &a, const AttnPart &p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.n_bh * p.row_tiles * p.n_split));
-    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DP, BY_ROWS, PREFIX>), grid, dim3(AttnTile<TK, TQ, DP, BY_ROWS, PREFIX>::WAVES * 64), 0, st, a, p);
+    attn_tiles<TK, TQ, DP, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
 }
 
 template <typename TK, typename TQ, int DP>
 static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
     const int G = a.H / a.Hk;
-    AttnPart p{};
-    p.slots = pl.slots;
+    AttnPart own{}, pre{};
+    own.slots = pl.slots;
     if (pl.slots > 1) {
-        const size_t rows = (size_t)a.B * a.H * a.n_q * pl.slots;
-        p.part_o = static_cast<float *>(work);
-        p.part_ml = p.part_o + rows * a.D;
+        own.part_o = static_cast<float *>(work);
+        own.part_ml = own.part_o + (size_t)a.B * a.H * a.n_q * pl.slots * a.D;
     }
+    pre = own;
     if (pl.pre_splits) {
-        p.slot0 = 0;
-        p.n_split = pl.pre_splits;
-        p.n_bh = a.Hk;
-        p.rows = a.B * a.n_q * G;
-        p.row_tiles = pl.pre_tiles;
-        if (pl.pre_rows) launch_tiles<TK, TQ, DP, true, true>(a, p, st);
-        else launch_tiles<TK, TQ, DP, false, true>(a, p, st);
+        pre.n_split = pl.pre_splits;
+        pre.n_bh = a.Hk;
+        pre.rows = a.B * a.n_q * G;
+        pre.row_tiles = pl.pre_tiles;
+        pre.blocks = pre.n_bh * pre.row_tiles * pre.n_split;
     }
-    p.slot0 = pl.slots - pl.own_splits;
-    p.n_split = pl.own_splits;
-    p.n_bh = a.B * a.Hk;
-    p.rows = a.n_q * G;
-    p.row_tiles = pl.own_tiles;
-    if (pl.own_rows) launch_tiles<TK, TQ, DP, true, false>(a, p, st);
-    else launch_tiles<TK, TQ, DP, false, false>(a, p, st);
-    if (pl.slots > 1) {
-        const int64_t rows = (int64_t)a.B * a.H * a.n_q;
-        hipLaunchKernelGGL((attn_join_kernel<TQ, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p);
+    own.slot0 = pl.pre_splits;
+    own.n_split = pl.own_splits;
+    own.n_bh = a.B * a.Hk;
+    own.rows = a.n_q * G;
+    own.row_tiles = pl.own_tiles;
+    own.blocks = own.n_bh * own.row_tiles * own.n_split;
+    const bool general = a.mask != nullptr || a.cap != 0.0f;
+    const dim3 grid((unsigned)(pre.blocks + own.blocks));
+#define ATTN_CASE(PRE, ROWS, GENERAL) hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DP, PRE, ROWS, GENERAL>), grid, dim3(256), 0, st, a, pre, own)
+    if (!pl.pre_splits) {
+        if (pl.own_rows) {
+            if (general) ATTN_CASE(0, true, true);
+            else ATTN_CASE(0, true, false);
+        } else {
+            if (general) ATTN_CASE(0, false, true);
+            else ATTN_CASE(0, false, false);
+        }
+    } else {
+        if (!pl.pre_rows) ATTN_CASE(1, false, false);
+        else if (!pl.own_rows) ATTN_CASE(2, false, false);
+        else ATTN_CASE(2, true, false);
     }
+#undef ATTN_CASE
+    if (pl.slots > 1) hipLaunchKernelGGL((attn_join_kernel<TQ, DP>), dim3((unsigned)(a.B * a.H * a.n_q)), dim3(256), 0, st, a, own);
 }
 
 template <typename TK, typename TQ>
@@ -907,76 +841,13 @@ static void launch_attn_d(const AttnArgs &a, const AttnPlan &pl, void *work, hip
     else launch_attn<TK, TQ, 256>(a, pl, work, st);
 }
 
-static bool has_data(const AttnTensors &t) {
-    return t.q.data && t.dst.data && (t.k.ne[1] == 0 || (t.k.data && t.v.data)) && (!t.kp || t.kp->ne[1] == 0 || (t.kp->data && t.vp->data)) &&
-           (!t.mask || t.mask->data) && (!t.sinks || t.sinks->data) && (!t.len || t.len->data);
+template <typename TK, typename TQ>
+static hipError_t launch_attn_any(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
+    if (pl.tiled) launch_attn_d<TK, TQ>(a, pl, work, st);
+    else hipLaunchKernelGGL((attn_rows_kernel<TQ, TK>), dim3(a.n_q, a.H, a.B), dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
-int flash_attn(const AttnTensors &t, const AttnSpec &p, hipStream_t st, Scratch &scratch) {
-    const int rc = check_attn(t, p);
-    if (rc != GGML_MI355X_OK) return rc;
-    const size_t bytes = flash_attn_work(t);
-    if (bytes == 0 || !has_data(t)) return flash_attn(t, p, nullptr, st);
-    std::lock_guard<std::mutex> hold(scratch.mu);   // until the kernels that use it are queued
-    void *work = scratch.get(bytes, st);
-    return work ? flash_attn(t, p, work, st) : GGML_MI355X_ENOMEM;
-}
-
-int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t st) {
-    const int rc = check_attn(t, p);
-    if (rc != GGML_MI355X_OK) return rc;
-    const TensorView &q = t.q, &k = t.k, &v = t.v, &d = t.dst;
-    if (q.ne[1] == 0 || q.ne[2] == 0 || q.ne[3] == 0) return GGML_MI355X_OK;
-    if (!has_data(t)) return GGML_MI355X_EINVAL;
-    AttnArgs a{};
-    a.q = static_cast<const char *>(q.data);
-    a.q_i = (int64_t)q.nb[1]; a.q_h = (int64_t)q.nb[2]; a.q_b = (int64_t)q.nb[3];
-    a.k = static_cast<const char *>(k.data);
-    a.k_j = (int64_t)k.nb[1]; a.k_h = (int64_t)k.nb[2]; a.k_b = (int64_t)k.nb[3];
-    a.v = static_cast<const char *>(v.data);
-    a.v_j = (int64_t)v.nb[1]; a.v_h = (int64_t)v.nb[2]; a.v_b = (int64_t)v.nb[3];
-    if (t.kp) {
-        a.kp = static_cast<const char *>(t.kp->data);
-        a.kp_j = (int64_t)t.kp->nb[1]; a.kp_h = (int64_t)t.kp->nb[2];
-        a.vp = static_cast<const char *>(t.vp->data);
-        a.vp_j = (int64_t)t.vp->nb[1]; a.vp_h = (int64_t)t.vp->nb[2];
-        a.n_prefix = (int)t.kp->ne[1];
-    }
-    if (t.mask) {
-        a.mask = static_cast<const char *>(t.mask->data);
-        a.m_i = (int64_t)t.mask->nb[1]; a.m_h = (int64_t)t.mask->nb[2]; a.m_b = (int64_t)t.mask->nb[3];
-        a.m_nh = (int)t.mask->ne[2]; a.m_nb = (int)t.mask->ne[3];
-        a.m_vec = aligned_to(*t.mask, 8);
-    }
-    if (t.sinks) a.sinks = static_cast<const float *>(t.sinks->data);
-    if (t.len) {
-        a.len = static_cast<const char *>(t.len->data);
-        a.len_b = (int64_t)t.len->nb[0];
-    }
-    a.o = static_cast<char *>(d.data);
-    a.o_h = (int64_t)d.nb[1]; a.o_i = (int64_t)d.nb[2]; a.o_b = (int64_t)d.nb[3];
-    a.D = (int)q.ne[0]; a.n_q = (int)q.ne[1]; a.n_kv = (int)k.ne[1];
-    a.H = (int)q.ne[2]; a.Hk = (int)k.ne[2]; a.B = (int)q.ne[3]; a.kv_b = (int)(q.ne[3] / k.ne[3]);
-    a.causal = p.causal;
-    a.scale = p.scale;
-    a.cap = p.logit_softcap;
-    if (p.max_bias > 0.0f) {
-        a.bias_heads = 1 << (int)std::floor(std::log2((double)a.H));
-        a.m0 = std::pow(2.0f, -p.max_bias / a.bias_heads);
-        a.m1 = std::pow(2.0f, -p.max_bias / 2.0f / a.bias_heads);
-    }
-    const AttnPlan pl = plan_attn(t);
-    if (pl.tiled) {
-        if (q.type == T_F32) launch_attn_d<_Float16, float>(a, pl, work, st);
-        else if (q.type == T_F16) launch_attn_d<_Float16, _Float16>(a, pl, work, st);
-        else launch_attn_d<__bf16, __bf16>(a, pl, work, st);
-    } else {
-        const dim3 grid(a.n_q, a.H, a.B);
-        if (q.type == T_F32) hipLaunchKernelGGL((attn_rows_kernel<float, _Float16>), grid, dim3(256), 0, st, a);
-        else if (q.type == T_F16) hipLaunchKernelGGL((attn_rows_kernel<_Float16, _Float16>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attn_rows_kernel<__bf16, __bf16>), grid, dim3(256), 0, st, a);
-    }
-    return hipGetLastError() == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
-}
+}  // namespace
 
 }  // namespace mi355x
