@@ -88,12 +88,27 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     for (const TensorView *x : {&t.k, &t.v, t.kp, t.vp})
         if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
     if (!p.tiled) return p;
-    auto pick = [](int64_t rows, int64_t problems, int64_t keys, bool &by_rows, int &tiles, int &splits) {
+    // Splits of the keys: the fewest us by a small model of the launch, with 512 workgroups at a time (2 a CU).
+    // us of a workgroup: 5 beside its tiles, and per tile of 64 keys by 128 rows 2.3 (measured: an 8192-token
+    // prompt's 132096 tiles in 604 us; twice that for f32 activations, half for heads of up to 64 values),
+    // per 128 keys of split keys 1.2. A split row costs the join a launch and its partial results a trip
+    // through memory.
+    const double D = (double)t.q.ne[0], size = (D <= 64 ? 0.5 : D <= 128 ? 1.0 : 2.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
+    auto pick = [&](int64_t rows, int64_t problems, int64_t keys, bool &by_rows, int &tiles, int &splits) {
         by_rows = rows > 32;
         tiles = (int)((rows + (by_rows ? 127 : 31)) / (by_rows ? 128 : 32));
-        const int64_t groups = std::max<int64_t>(1, problems * tiles);
-        splits = (int)std::max<int64_t>(1, std::min({(512 + groups - 1) / groups, (keys + 127) / 128, (int64_t)ATTN_MAX_SLOTS / 2}));
-        if (groups >= 256) splits = 1;
+        const double groups = (double)std::max<int64_t>(1, problems * tiles), steps = std::ceil(keys / 128.0);
+        double best = 0.0;
+        splits = 1;
+        for (int s = 1; s <= ATTN_MAX_SLOTS / 2 && (s == 1 || s <= steps); ++s) {
+            const double rounds = std::ceil(groups * s / 512.0), n = std::ceil(steps / s);
+            double us = rounds * (5.0 + n * (by_rows ? 2 * 2.3 * size : 1.2));
+            if (s > 1 || t.kp) us += 4.0 + problems * rows * s * D * 8 / 4e6;
+            if (s == 1 || us < best) {
+                best = us;
+                splits = s;
+            }
+        }
     };
     pick(n_q * G, B * Hk, t.k.ne[1], p.own_rows, p.own_tiles, p.own_splits);
     p.slots = p.own_splits;

@@ -24,6 +24,15 @@ __device__ __forceinline__ float wave_add(float v) {
     return v;
 }
 
+// tanh without a branch: below 1/4 the odd Taylor polynomial to x^9 (the next term is 2^-26 of x there), above
+// (1 - t) / (1 + t), t = exp(-2 |x|); off by some 3 units in the last place
+__device__ __forceinline__ float tanh_of(float x) {
+    const float y = fabsf(x), t = __builtin_amdgcn_exp2f(-2.0f * LOG2E * y), q = x * x;
+    const float big = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+    const float odd = fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return y < 0.25f ? x * odd : big;   // (a NaN fails the comparison and comes out of `big`)
+}
+
 __device__ __forceinline__ float slope_of(const AttnArgs &a, int h) {
     if (a.bias_heads == 0) return 1.0f;
     return h < a.bias_heads ? powf(a.m0, (float)(h + 1)) : powf(a.m1, (float)(2 * (h - a.bias_heads) + 1));
@@ -32,7 +41,7 @@ __device__ __forceinline__ float slope_of(const AttnArgs &a, int h) {
 // a score in units of log 2: the cap and the factor log2(e), so that exp is one exp2
 __device__ __forceinline__ float scaled(const AttnArgs &a, float s) {
     s *= a.scale;
-    if (a.cap != 0.0f) s = a.cap * tanhf(s / a.cap);
+    if (a.cap != 0.0f) s = a.cap * tanh_of(s / a.cap);
     return s * LOG2E;
 }
 
@@ -384,50 +393,56 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p,
     }
 }
 
-// the splits' partial results of a row: a workgroup a row, groups of DP / 4 threads take every GROUPS-th
-// split and are joined in their order
-template <typename TQ, int DP>
+// the splits' partial results of a row, joined in a fixed order: GROUPS groups of DP / 4 threads a row take
+// every GROUPS-th split
+template <typename TQ, int DP, int GROUPS>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a, const AttnPart p) {
-    constexpr int LPR = DP / 4, GROUPS = 256 / LPR;
-    __shared__ float weight[ATTN_MAX_SLOTS];
-    __shared__ f32x4 part[GROUPS][LPR];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t rr = blockIdx.x;
+    constexpr int LPR = DP / 4, TPR = LPR * GROUPS, ROWS = 256 / TPR;
+    __shared__ f32x4 part[ROWS][GROUPS == 1 ? 1 : GROUPS][GROUPS == 1 ? 1 : LPR];
+    const int tid = threadIdx.x, row = tid / TPR, grp = tid % TPR / LPR, d = tid % LPR * 4;
+    const int64_t rows = (int64_t)a.B * a.H * a.n_q, rr = min((int64_t)blockIdx.x * ROWS + row, rows - 1);
     const int G = a.H / a.Hk, per = a.n_q * G;
     const int r = (int)(rr % per), hk = (int)(rr / per % a.Hk), b = (int)(rr / per / a.Hk), i = r / G, head = hk * G + r % G;
-    const int d = tid % LPR * 4, grp = tid / LPR;
-    const float *po = p.part_o + rr * p.slots * a.D + d;
-    // (at most ATTN_MAX_SLOTS / GROUPS values a thread: the first ones are on their way while the weights form)
+    const float *po = p.part_o + rr * p.slots * a.D + d, *ml = p.part_ml + 2 * rr * p.slots;
+    const bool has = d < a.D;
+    // (the first two of the thread's splits are on their way while the maximum forms)
     f32x4 x0{}, x1{};
-    if (d < a.D) {
-        if (grp < p.slots) x0 = *reinterpret_cast<const f32x4 *>(po + (int64_t)grp * a.D);
-        if (grp + GROUPS < p.slots) x1 = *reinterpret_cast<const f32x4 *>(po + (int64_t)(grp + GROUPS) * a.D);
-    }
-    const float *ml = p.part_ml + 2 * rr * p.slots;
-    float m = -INFINITY;   // (every wave looks at all of them)
-    for (int s = lane; s < p.slots; s += 64) m = fmaxf(m, ml[2 * s]);
+    if (has && grp < p.slots) x0 = *reinterpret_cast<const f32x4 *>(po + (int64_t)grp * a.D);
+    if (has && grp + GROUPS < p.slots) x1 = *reinterpret_cast<const f32x4 *>(po + (int64_t)(grp + GROUPS) * a.D);
+    float m = -INFINITY, l = 0.0f;
+    auto weight_of = [&](int s) { return m == -INFINITY ? 1.0f : exp2f(ml[2 * s] - m); };
+    __shared__ float weights[GROUPS == 1 ? 1 : ATTN_MAX_SLOTS];
+    if constexpr (GROUPS == 1) {   // a few splits
+        for (int s = 0; s < p.slots; ++s) m = fmaxf(m, ml[2 * s]);
+        for (int s = 0; s < p.slots; ++s) l += ml[2 * s + 1] * weight_of(s);
+    } else {                       // one row a workgroup: every wave looks at all of them
+        const int lane = tid & 63;
+        for (int s = lane; s < p.slots; s += 64) m = fmaxf(m, ml[2 * s]);
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    float l = 0.0f;
-    for (int s = lane; s < p.slots; s += 64) {
-        const float f = m == -INFINITY ? 1.0f : exp2f(ml[2 * s] - m);
-        if (tid < 64) weight[s] = f;
-        l += ml[2 * s + 1] * f;
+        for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+        for (int s = lane; s < p.slots; s += 64) {
+            const float f = weight_of(s);
+            if (tid < 64) weights[s] = f;
+            l += ml[2 * s + 1] * f;
+        }
+        l = wave_add(l);
+        __syncthreads();
     }
-    l = wave_add(l);
-    __syncthreads();
+    auto weight = [&](int s) { return GROUPS == 1 ? weight_of(s) : weights[s]; };
     f32x4 x{};
-    if (grp < p.slots) x += x0 * weight[grp];
-    if (grp + GROUPS < p.slots) x += x1 * weight[grp + GROUPS];
-    if (d < a.D) {
+    if (grp < p.slots) x += x0 * weight(grp);
+    if (grp + GROUPS < p.slots) x += x1 * weight(grp + GROUPS);
+    if (has) {
 #pragma unroll 4
-        for (int s = grp + 2 * GROUPS; s < p.slots; s += GROUPS) x += *reinterpret_cast<const f32x4 *>(po + (int64_t)s * a.D) * weight[s];
+        for (int s = grp + 2 * GROUPS; s < p.slots; s += GROUPS) x += *reinterpret_cast<const f32x4 *>(po + (int64_t)s * a.D) * weight(s);
     }
-    part[grp][tid % LPR] = x;
-    __syncthreads();
-    if (grp != 0 || d >= a.D) return;
-    const int most = min(GROUPS, p.slots);
-    for (int g = 1; g < most; ++g) x += part[g][tid];
+    if constexpr (GROUPS > 1) {
+        part[row][grp][tid % LPR] = x;
+        __syncthreads();
+    }
+    if (grp != 0 || !has || (int64_t)blockIdx.x * ROWS + row >= rows) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) x += part[row][g][tid % LPR];   // (by the row's first group, in order)
     TQ *out = reinterpret_cast<TQ *>(a.o + i * a.o_i + head * a.o_h + b * a.o_b);
     store4<TQ>(out + d, x * finish(a, head, m, l));
 }
@@ -482,7 +497,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     float slope = 0.0f;
     if (masked) {
         mrow = a.mask + i * a.m_i + (head % a.m_nh) * a.m_h + (b % a.m_nb) * a.m_b;
-        slope = slope_of(a, head) * LOG2E;
+        // (above 0, so that -inf stays -inf; a hidden key whose product is not finite makes the row NaN, and the
+        // row is done again)
+        slope = fmaxf(slope_of(a, head) * LOG2E, 0x1p-100f);
     }
 
     const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + (int64_t)(pb / a.kv_b) * a.k_b;
@@ -598,6 +615,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         }
     };
 
+    // LDS reads run AHEAD operands ahead of the MFMAs that take them: left to itself the compiler, short of
+    // registers, reads each operand right before its use
+    constexpr int AHEAD = 4, PER = SPLIT ? 2 : 1;   // (MFMAs an operand)
     f32x16 s[KT / 32];
     auto products = [&](const char *kt) {
         const int krow = lane & 31, ksw = swz_k<DP>(krow);
@@ -611,6 +631,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 if constexpr (SPLIT) s[u] = mma(kf, ql[t], s[u]);
             }
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int n = AHEAD; n < KT / 32 * NT; ++n) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, PER * AHEAD, 0);
     };
     // the weights of the tile's keys from their products: s[u][r] belongs to key j + 32 u + 8 (r / 4) + 4 h +
     // r % 4, f times it is the score in units of log 2
@@ -618,19 +645,24 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         const int left = seen - j - 4 * h;
         float f = c;
         if (capped || masked) {
+            const float by = capped ? c_cap : c;
             f = 1.0f;
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float x = s[u][r];
-                    x = capped ? cap2 * tanhf(x * c_cap) : x * c;
-                    if (masked) {
-                        const float add = (float)w[4 * u + r / 4][r % 4];
-                        x = add == -INFINITY ? -INFINITY : fmaf(slope, add, x);
-                    }
-                    s[u][r] = x;
-                }
+                for (int r = 0; r < 16; ++r) s[u][r] *= by;
+        }
+        if (capped) {
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = cap2 * tanh_of(s[u][r]);
+        }
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = fmaf(slope, (float)w[4 * u + r / 4][r % 4], s[u][r]);
         }
         if (__any(seen - j < KT)) {
 #pragma unroll
@@ -687,6 +719,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 if constexpr (SPLIT) o[d] = mma(vf, pl, o[d]);
             }
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 1);
+#pragma unroll
+        for (int n = AHEAD; n < KT / 16 * NB; ++n) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PER, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, PER * AHEAD, 1);
     };
 
     if constexpr (BY_ROWS) {
@@ -778,8 +817,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 // One launch: the workgroups of a shared prefix (PRE: 0 none, 1 split keys, 2 row tiles), which are bound
 // by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs
 template <typename TK, typename TQ, int DP, int PRE, bool OWN_ROWS, bool GENERAL>
-__global__ __launch_bounds__(256, DP == 256 || (DP == 128 && GENERAL && sizeof(TQ) == 4) ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre,
-                                                                                                    const AttnPart own) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
     constexpr int L0 = AttnTile<TK, TQ, DP, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DP, PRE == 2>::LDS;
     __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
     if constexpr (PRE != 0) {
@@ -831,7 +869,18 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
         else ATTN_CASE(2, true, false);
     }
 #undef ATTN_CASE
-    if (pl.slots > 1) hipLaunchKernelGGL((attn_join_kernel<TQ, DP>), dim3((unsigned)(a.B * a.H * a.n_q)), dim3(256), 0, st, a, own);
+    if (pl.slots > 1) {
+        // a row's splits side by side (8 of them with 128 values a row, at most 8 a thread then) where rows are
+        // few; one group of threads a row where a row has a few splits or its rows fill the CUs by themselves
+        const int64_t rows = (int64_t)a.B * a.H * a.n_q;
+        constexpr int ALL = 1024 / DP;
+        if (pl.slots <= 2 || (pl.slots <= 8 && rows >= 8192)) {
+            const unsigned grid = (unsigned)((rows * (DP / 4) + 255) / 256);
+            hipLaunchKernelGGL((attn_join_kernel<TQ, DP, 1>), dim3(grid), dim3(256), 0, st, a, own);
+        } else {
+            hipLaunchKernelGGL((attn_join_kernel<TQ, DP, ALL>), dim3((unsigned)rows), dim3(256), 0, st, a, own);
+        }
+    }
 }
 
 template <typename TK, typename TQ>
