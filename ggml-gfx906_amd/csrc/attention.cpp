@@ -88,34 +88,64 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     for (const TensorView *x : {&t.k, &t.v, t.kp, t.vp})
         if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
     if (!p.tiled) return p;
-    // Splits of the keys: the fewest us by a small model of the launch, with 512 workgroups at a time (2 a CU).
-    // us of a workgroup: 5 beside its tiles, and per tile of 64 keys by 128 rows 2.3 (measured: an 8192-token
-    // prompt's 132096 tiles in 604 us; twice that for f32 activations, half for heads of up to 64 values),
-    // per 128 keys of split keys 1.2. A split row costs the join a launch and its partial results a trip
-    // through memory.
-    const double D = (double)t.q.ne[0], size = (D <= 64 ? 0.5 : D <= 128 ? 1.0 : 2.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
-    auto pick = [&](int64_t rows, int64_t problems, int64_t keys, bool &by_rows, int &tiles, int &splits) {
-        by_rows = rows > 32;
-        tiles = (int)((rows + (by_rows ? 127 : 31)) / (by_rows ? 128 : 32));
-        const double groups = (double)std::max<int64_t>(1, problems * tiles), steps = std::ceil(keys / 128.0);
-        double best = 0.0;
-        splits = 1;
-        for (int s = 1; s <= ATTN_MAX_SLOTS / 2 && (s == 1 || s <= steps); ++s) {
-            const double rounds = std::ceil(groups * s / 512.0), n = std::ceil(steps / s);
-            double us = rounds * (5.0 + n * (by_rows ? 2 * 2.3 * size : 1.2));
-            if (s > 1 || t.kp) us += 4.0 + problems * rows * s * D * 8 / 4e6;
-            if (s == 1 || us < best) {
-                best = us;
-                splits = s;
+    // Splits of the keys, and workgroups of 4 or of 8 waves: the fewest us by a model of the launch.
+    //   a workgroup: 5 us beside its tiles, then, per tile of 64 keys, by row tiles 1.7 alone on its CU and 2.3
+    //     beside another one (4 waves, 128 rows), 2.15 with 8 waves (256 rows; measured: an 8192-token prompt's
+    //     132096 and 66048 tiles in 591 and 544 us); half for heads of up to 64 values, twice for f32
+    //     activations. With split keys 1.2 per 32 keys of every wave
+    //   the launch: its longest workgroup, or all of them over the workgroups that run at once and, for
+    //     split keys, their bytes at 5.5 TB/s
+    //   more than one partial result a row: 4 for the second launch, and their trip through memory
+    // (64 sequences behind 8192 keys: 65 / 44 / 49 / 53 us with 4 / 8 / 16 / 32 splits of the prefix, the model
+    // says 65 / 40 / 43 / 49; one token on 1000 keys, 12 heads: 13.8 / 11.1 with 1 / 8, the model 14.6 / 10.2.)
+    struct Part { double longest, all; int tiles; };
+    const int64_t D = t.q.ne[0], rows = n_q * G;
+    const double size = (D <= 64 ? 0.5 : 1.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
+    auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int s, bool whole_rounds) {
+        const int64_t per_tile = by_rows ? waves * 32 : 32, step = by_rows ? (D <= 128 ? 64 : 32) : waves * 32;
+        const int tiles = (int)((rows + per_tile - 1) / per_tile);
+        const double groups = (double)problems * tiles * s, n = std::ceil(std::ceil((double)keys / s) / step);
+        const double at_once = D > 128 || (waves == 8 && (by_rows || D > 64)) ? 256.0 : 512.0;
+        const double rounds = whole_rounds ? std::ceil(groups / at_once) : groups / at_once;
+        if (by_rows) {
+            const double alone = (waves == 8 ? 2.15 : 1.7) * size, beside = (waves == 8 ? 2.15 : 2.3) * size;
+            return Part{5.0 + n * alone, rounds * (5.0 + n * beside), tiles};
+        }
+        return Part{5.0 + n * 1.2, groups / at_once * 5.0 + (double)problems * keys * D * 4 / 5.5e6, tiles};
+    };
+    static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+    static_assert(128 <= ATTN_MAX_SLOTS / 2, "a prefix's splits and the batches' own");
+    const int wide = D <= 128 ? 8 : 4;
+    p.own_rows = rows > 32;
+    p.pre_rows = t.kp && B * rows > 32;
+    double best = 0.0;
+    auto join = [&](int slots) { return slots > 1 ? 4.0 + (double)B * H * n_q * slots * D * 8 / 8e6 : 0.0; };
+    auto take = [&](int waves, int own, const Part &o, int pre, const Part &r) {
+        const double us = std::max({o.longest, r.longest, o.all + r.all}) + join(own + pre);
+        if (p.slots != 0 && us >= best) return;
+        best = us;
+        p.waves = waves;
+        p.own_splits = own;
+        p.own_tiles = o.tiles;
+        p.pre_splits = pre;
+        p.pre_tiles = r.tiles;
+        p.slots = own + pre;
+    };
+    const int64_t n_kv = t.k.ne[1], n_pre = t.kp ? t.kp->ne[1] : 0;
+    // (two sets of row tiles gain by the wide workgroups; beside a memory-bound part two smaller ones do)
+    for (int waves = t.kp && p.own_rows ? wide : 4; waves <= (t.kp && !p.own_rows ? 4 : wide); waves += 4)
+        for (int so : SPLITS) {
+            if (so > 1 && (so - 1) * 32 >= n_kv) break;
+            const Part o = part(rows, B * Hk, n_kv, p.own_rows, waves, so, !t.kp);
+            if (!t.kp) {
+                take(waves, so, o, 0, Part{0.0, 0.0, 0});
+                continue;
+            }
+            for (int sp : SPLITS) {
+                if (sp > 1 && (sp - 1) * 32 >= n_pre) break;
+                take(waves, so, o, sp, part(B * rows, Hk, n_pre, p.pre_rows, waves, sp, false));
             }
         }
-    };
-    pick(n_q * G, B * Hk, t.k.ne[1], p.own_rows, p.own_tiles, p.own_splits);
-    p.slots = p.own_splits;
-    if (t.kp) {
-        pick(B * n_q * G, Hk, t.kp->ne[1], p.pre_rows, p.pre_tiles, p.pre_splits);
-        p.slots += p.pre_splits;
-    }
     return p;
 }
 
@@ -183,9 +213,12 @@ int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t 
         a.m1 = std::pow(2.0f, -p.max_bias / 2.0f / a.bias_heads);
     }
     const AttnPlan pl = plan_attn(t);
-    const hipError_t e = q.type == T_F32   ? attn_launch_f16_f32(a, pl, work, st)
-                         : q.type == T_F16 ? attn_launch_f16(a, pl, work, st)
-                                           : attn_launch_bf16(a, pl, work, st);
+    typedef hipError_t (*Launch)(const AttnArgs &, const AttnPlan &, void *, hipStream_t);
+    static const Launch launch[3][3] = {{attn_launch_f16_64, attn_launch_f16_128, attn_launch_f16_256},
+                                        {attn_launch_bf16_64, attn_launch_bf16_128, attn_launch_bf16_256},
+                                        {attn_launch_f32_64, attn_launch_f32_128, attn_launch_f32_256}};
+    const int type = q.type == T_F32 ? 2 : q.type == T_BF16 ? 1 : 0;
+    const hipError_t e = launch[type][a.D <= 64 ? 0 : a.D <= 128 ? 1 : 2](a, pl, work, st);
     return e == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
 }
 

@@ -30,14 +30,23 @@ constexpr int ATTN_MAX_SLOTS = 256;   // partial results of a row
 // what a call launches, by its shapes alone
 struct AttnPlan {
     bool tiled;                              // else attn_rows_kernel
-    bool own_rows, pre_rows;                 // row tiles of 128 (4 waves of 32), or 32 rows with split keys
+    int waves;                               // of a workgroup
+    bool own_rows, pre_rows;                 // row tiles of 32 per wave, or 32 rows whose keys the waves split
     int own_tiles, own_splits, pre_tiles, pre_splits, slots;
 };
 
-// the launches of one call: cache type, then activation type (attention_f16.hip, attention_bf16.hip,
-// attention_f32.hip). `work`: the partial results of pl.slots > 1
-hipError_t attn_launch_f16(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st);
-hipError_t attn_launch_bf16(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st);
-hipError_t attn_launch_f16_f32(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st);
+// the launches of one call, by cache and activation type and by the head size the kernels are built for (D up
+// to it; attention_kernels.hip). `work`: the partial results of pl.slots > 1
+#define ATTN_LAUNCH(NAME) hipError_t NAME(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st);
+ATTN_LAUNCH(attn_launch_f16_64)
+ATTN_LAUNCH(attn_launch_f16_128)
+ATTN_LAUNCH(attn_launch_f16_256)
+ATTN_LAUNCH(attn_launch_bf16_64)
+ATTN_LAUNCH(attn_launch_bf16_128)
+ATTN_LAUNCH(attn_launch_bf16_256)
+ATTN_LAUNCH(attn_launch_f32_64)
+ATTN_LAUNCH(attn_launch_f32_128)
+ATTN_LAUNCH(attn_launch_f32_256)
+#undef ATTN_LAUNCH
 
 }  // namespace mi355x

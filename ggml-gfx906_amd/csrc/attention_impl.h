@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // running maximum and sum are the lane's own scalars, and they are the very values that O^T's B operand
 // wants from that lane once the keys are taken in the order the MFMA returned them: the weights never
 // leave the registers. Tiles come by LDS DMA, one tile ahead.
-//   BY_ROWS: 4 waves of 32 rows each share tiles of KT keys (prompts, shared prefixes)
-//   else:    4 waves share 32 rows and take tiles of 32 keys in turn, joined at the end (tokens)
+//   BY_ROWS: 4 or 8 waves of 32 rows each share tiles of KT keys (prompts, shared prefixes)
+//   else:    4 or 8 waves share 32 rows and take tiles of 32 keys in turn, joined at the end (tokens)
 // 16-byte pieces of a tile's rows are permuted (swz_k, swz_v) so that neither read meets an LDS bank
 // twice; the DMA writes LDS in order, so the permutation is in the addresses it reads from.
 //
@@ -199,19 +199,20 @@ __device__ __forceinline__ void dma16(i32x4 r, const char *dst, uint32_t voff, u
                  :: "s"(at), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
 
-template <typename TK, typename TQ, int DP, bool BY_ROWS>
+template <typename TK, typename TQ, int DP, int WAVES, bool BY_ROWS>
 struct AttnTile {
     static constexpr bool SPLIT = sizeof(TQ) == 4;
     static constexpr int KT = BY_ROWS && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int CPR = DP / 8;                          // 16-byte pieces of a row
-    static constexpr int LOADERS = BY_ROWS ? 256 : 64;          // threads that load a tile together
+    static constexpr int LOADERS = BY_ROWS ? WAVES * 64 : 64;   // threads that load a tile together
     static constexpr int RPI = LOADERS / CPR;                   // rows of one DMA round
     static constexpr int ROUNDS = KT / RPI;
     static constexpr int BYTES = KT * DP * 2;                   // of a tile of keys, and of values
     // BY_ROWS: two stages of keys and values; else one of each per wave, whose 32 rows also fit it as f32,
     // and those rows' maxima and sums
     static constexpr int STRETCH = BY_ROWS ? 4 * BYTES : 2 * BYTES + 256;
-    static constexpr int LDS = (BY_ROWS ? 1 : 4) * STRETCH;
+    static constexpr int LDS = (BY_ROWS ? 1 : WAVES) * STRETCH;
+    static constexpr int STEP = BY_ROWS ? KT : WAVES * 32;      // keys that a workgroup takes at a time
     typedef typename Vec<TK>::x8 x8;
 };
 
@@ -331,12 +332,12 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
     }
 }
 
-// 32 rows that the four waves hold parts of, each in its stretch of LDS (values [row][DP], then the
-// maxima and the sums): 8 threads a row
-template <typename TK, typename TQ, int DP, bool PREFIX>
+// 32 rows that the waves hold parts of, each in its stretch of LDS (values [row][DP], then the maxima and
+// the sums): two threads of each wave a row
+template <typename TK, typename TQ, int DP, int WAVES, bool PREFIX>
 __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p, const char *lds, int stretch, int tops, int row0, int bh,
                                            int split, int j_begin, int j_end) {
-    constexpr int WAVES = 4, TPR = 8, N = DP / TPR;
+    constexpr int TPR = WAVES * 2, N = DP / TPR;
     const int r = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N, row = row0 + r;
     const bool ok = row < p.rows;
     float m = -INFINITY, l = 0.0f, f[WAVES];
@@ -454,9 +455,9 @@ __device__ __forceinline__ uint32_t piece_off(int place, int swz, int D) { retur
 // have no mask, and may have a cap)
 enum AttnKind { OWN, OWN_GENERAL, OWN_BEHIND, PREFIX_KEYS };
 
-template <typename TK, typename TQ, int DP, bool BY_ROWS, AttnKind KIND>
+template <typename TK, typename TQ, int DP, int WAVES, bool BY_ROWS, AttnKind KIND>
 __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p, char *lds, int id) {
-    using T = AttnTile<TK, TQ, DP, BY_ROWS>;
+    using T = AttnTile<TK, TQ, DP, WAVES, BY_ROWS>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
     constexpr int KT = T::KT, CPR = T::CPR, RPI = T::RPI, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DP / 16, NB = DP / 32;
@@ -468,7 +469,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int G = a.H / a.Hk, hk = bh % a.Hk, pb = bh / a.Hk;
 
     // this lane's row
-    const int row0 = BY_ROWS ? tile * 128 + wave * 32 : tile * 32;
+    const int row0 = (BY_ROWS ? tile * WAVES + wave : tile) * 32;
     const int row = min(row0 + (lane & 31), p.rows - 1);
     const bool row_ok = row0 + (lane & 31) < p.rows;
     const int g = row % G, bi = row / G;
@@ -479,12 +480,12 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int n = PREFIX ? a.n_prefix : own_len(a, b);
     int end = n;                                    // of the workgroup's rows
     if (!PREFIX && a.causal) {
-        const int last = min(BY_ROWS ? tile * 128 + 127 : row0 + 31, p.rows - 1) / G;
+        const int last = min((BY_ROWS ? (tile + 1) * WAVES : tile + 1) * 32 - 1, p.rows - 1) / G;
         end = max(0, n - a.n_q + last + 1);
     }
     int j_begin = 0, j_end = end;
     if (p.n_split > 1) {
-        const int per = ((end + p.n_split - 1) / p.n_split + 127) & ~127;
+        const int per = ((end + p.n_split - 1) / p.n_split + T::STEP - 1) / T::STEP * T::STEP;
         j_begin = min(end, split * per);
         j_end = min(end, j_begin + per);
     }
@@ -750,9 +751,14 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 if (masked) fetch(j + KT, ahead);
             }
             if (j < seen_most) {
+                // (a wave that feeds the matrix cores goes before one that forms weights)
+                __builtin_amdgcn_s_setprio(1);
                 products(now);
+                __builtin_amdgcn_s_setprio(0);
                 weights(j, w);
+                __builtin_amdgcn_s_setprio(1);
                 values(now + BYTES);
+                __builtin_amdgcn_s_setprio(0);
             }
             char *t = now;
             now = next;
@@ -761,7 +767,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     } else {
         // a tile's keys are refilled once their products are formed, its values behind those, so that either
         // is on its way while the other is worked on
-        constexpr int STEP = 4 * 32;
+        constexpr int STEP = T::STEP;
         f16x4 w[KT / 8], ahead[KT / 8];
         if (masked && j0 < j_end) fetch(j0, ahead);
         for (int j = j0; j < j_end; j += STEP) {
@@ -808,25 +814,27 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             pm[32 + lane] = l;
         }
         __syncthreads();
-        join_waves<TK, TQ, DP, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
+        join_waves<TK, TQ, DP, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
     } else {
         store_rows<TK, TQ, DP, PREFIX>(a, p, o, me, l, row, row_ok, bh, split, j_begin, j_end);
     }
 }
 
 // One launch: the workgroups of a shared prefix (PRE: 0 none, 1 split keys, 2 row tiles), which are bound
-// by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs
-template <typename TK, typename TQ, int DP, int PRE, bool OWN_ROWS, bool GENERAL>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
-    constexpr int L0 = AttnTile<TK, TQ, DP, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DP, PRE == 2>::LDS;
+// by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs. 8 waves on a
+// CU: two workgroups of 4, which take turns at the matrix cores, or one of 8, which loads each tile of keys
+// for twice the rows; 4 where the largest heads' accumulators leave room for no more.
+template <typename TK, typename TQ, int DP, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL>
+__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
+    constexpr int L0 = AttnTile<TK, TQ, DP, WAVES, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DP, WAVES, PRE == 2>::LDS;
     __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
     if constexpr (PRE != 0) {
         if ((int)blockIdx.x < pre.blocks) {
-            attn_tiles<TK, TQ, DP, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
+            attn_tiles<TK, TQ, DP, WAVES, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
             return;
         }
     }
-    attn_tiles<TK, TQ, DP, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
+    attn_tiles<TK, TQ, DP, WAVES, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
 }
 
 template <typename TK, typename TQ, int DP>
@@ -854,19 +862,23 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     own.blocks = own.n_bh * own.row_tiles * own.n_split;
     const bool general = a.mask != nullptr || a.cap != 0.0f;
     const dim3 grid((unsigned)(pre.blocks + own.blocks));
-#define ATTN_CASE(PRE, ROWS, GENERAL) hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DP, PRE, ROWS, GENERAL>), grid, dim3(256), 0, st, a, pre, own)
-    if (!pl.pre_splits) {
-        if (pl.own_rows) {
-            if (general) ATTN_CASE(0, true, true);
-            else ATTN_CASE(0, true, false);
-        } else {
-            if (general) ATTN_CASE(0, false, true);
-            else ATTN_CASE(0, false, false);
-        }
+    constexpr int WIDE = DP == 256 ? 4 : 8;
+#define ATTN_CASE(WAVES, PRE, ROWS, GENERAL) \
+    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DP, WAVES, PRE, ROWS, GENERAL>), grid, dim3(WAVES * 64), 0, st, a, pre, own)
+    if (pl.pre_splits) {
+        if (!pl.pre_rows) ATTN_CASE(4, 1, false, false);
+        else if (!pl.own_rows) ATTN_CASE(4, 2, false, false);
+        else ATTN_CASE(WIDE, 2, true, false);
+    } else if (pl.waves == 4) {
+        if (pl.own_rows && general) ATTN_CASE(4, 0, true, true);
+        else if (pl.own_rows) ATTN_CASE(4, 0, true, false);
+        else if (general) ATTN_CASE(4, 0, false, true);
+        else ATTN_CASE(4, 0, false, false);
     } else {
-        if (!pl.pre_rows) ATTN_CASE(1, false, false);
-        else if (!pl.own_rows) ATTN_CASE(2, false, false);
-        else ATTN_CASE(2, true, false);
+        if (pl.own_rows && general) ATTN_CASE(WIDE, 0, true, true);
+        else if (pl.own_rows) ATTN_CASE(WIDE, 0, true, false);
+        else if (general) ATTN_CASE(WIDE, 0, false, true);
+        else ATTN_CASE(WIDE, 0, false, false);
     }
 #undef ATTN_CASE
     if (pl.slots > 1) {
@@ -883,16 +895,9 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     }
 }
 
-template <typename TK, typename TQ>
-static void launch_attn_d(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
-    if (a.D <= 64) launch_attn<TK, TQ, 64>(a, pl, work, st);
-    else if (a.D <= 128) launch_attn<TK, TQ, 128>(a, pl, work, st);
-    else launch_attn<TK, TQ, 256>(a, pl, work, st);
-}
-
-template <typename TK, typename TQ>
+template <typename TK, typename TQ, int DP>
 static hipError_t launch_attn_any(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
-    if (pl.tiled) launch_attn_d<TK, TQ>(a, pl, work, st);
+    if (pl.tiled) launch_attn<TK, TQ, DP>(a, pl, work, st);
     else hipLaunchKernelGGL((attn_rows_kernel<TQ, TK>), dim3(a.n_q, a.H, a.B), dim3(256), 0, st, a);
     return hipGetLastError();
 }
