@@ -89,61 +89,70 @@ static AttnPlan plan_attn(const AttnTensors &t) {
         if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
     if (!p.tiled) return p;
     // Splits of the keys, and workgroups of 4 or of 8 waves: the fewest us by a model of the launch.
-    //   a workgroup: 5 us beside its tiles, then, per tile of 64 keys, by row tiles 1.7 alone on its CU and 2.3
-    //     beside another one (4 waves, 128 rows), 2.15 with 8 waves (256 rows; measured: an 8192-token prompt's
-    //     132096 and 66048 tiles in 591 and 544 us); half for heads of up to 64 values, twice for f32
-    //     activations. With split keys 1.2 per 32 keys of every wave
-    //   the launch: its longest workgroup, or all of them over the workgroups that run at once and, for
-    //     split keys, their bytes at 5.5 TB/s
+    //   a workgroup of row tiles: 7 us (8 waves: 9), and per tile of 64 keys 1.7 alone on its CU, 2.3 beside another
+    //     one (4 waves, 128 rows), 2.25 with 8 waves (256 rows); half for heads of up to 64 values, twice for f32
+    //     activations
+    //   a workgroup of split keys: 5 us, and per 128 keys what one CU draws from HBM, 1.6 (1.1 up to 64 values); all
+    //     of them no less than their bytes at 5.5 TB/s, which fewer than 256 workgroups do not reach
+    //   a prefix's workgroups are dealt first, then the batches' own, 512 (256 wide ones) at a time
     //   more than one partial result a row: 4 for the second launch, and their trip through memory
-    // (64 sequences behind 8192 keys: 65 / 44 / 49 / 53 us with 4 / 8 / 16 / 32 splits of the prefix, the model
-    // says 65 / 40 / 43 / 49; one token on 1000 keys, 12 heads: 13.8 / 11.1 with 1 / 8, the model 14.6 / 10.2.)
-    struct Part { double longest, all; int tiles; };
+    // Measured / by the model, us: one token, 8 key heads of 128 values, 8192 keys, 1 / 4 / 16 / 32 / 64 splits 85.7,
+    // 30.9, 17.2, 16.9, 19.2 / 107, 35, 17, 18, 21; 131072 keys, 16 / 24 / 32 / 64 splits 122, 116, 105, 106 / 131, 119,
+    // 110, 116; 64 sequences behind 8192 shared keys, 6 / 8 / 16 splits of them 54, 46, 53 / 65, 52, 58; 16 x 4 draft
+    // tokens behind 32768, 24 / 28 / 32 splits 62, 58, 68 / 72, 72, 79.
     const int64_t D = t.q.ne[0], rows = n_q * G;
     const double size = (D <= 64 ? 0.5 : 1.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
-    auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int s, bool whole_rounds) {
-        const int64_t per_tile = by_rows ? waves * 32 : 32, step = by_rows ? (D <= 128 ? 64 : 32) : waves * 32;
+    struct Part { double groups, alone, beside, bytes; int tiles; };   // workgroups, us of each, bytes of split keys
+    auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int s) {
+        const int64_t per_tile = by_rows ? waves * 32 : 32, step = by_rows ? (D <= 128 ? 64 : 32) : 128;
         const int tiles = (int)((rows + per_tile - 1) / per_tile);
         const double groups = (double)problems * tiles * s, n = std::ceil(std::ceil((double)keys / s) / step);
-        const double at_once = D > 128 || (waves == 8 && (by_rows || D > 64)) ? 256.0 : 512.0;
-        const double rounds = whole_rounds ? std::ceil(groups / at_once) : groups / at_once;
-        if (by_rows) {
-            const double alone = (waves == 8 ? 2.15 : 1.7) * size, beside = (waves == 8 ? 2.15 : 2.3) * size;
-            return Part{5.0 + n * alone, rounds * (5.0 + n * beside), tiles};
-        }
-        return Part{5.0 + n * 1.2, groups / at_once * 5.0 + (double)problems * keys * D * 4 / 5.5e6, tiles};
+        if (!by_rows) return Part{groups, 5.0 + n * (D <= 64 ? 1.1 : 1.6), 0.0, (double)problems * keys * D * 4, tiles};
+        if (waves == 8) return Part{groups, 9.0 + n * 2.25 * size, 9.0 + n * 2.25 * size, 0.0, tiles};
+        return Part{groups, 7.0 + n * 1.7 * size, 7.0 + n * 2.3 * size, 0.0, tiles};
     };
-    static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+    auto launch = [&](const Part &pre, const Part &own, int waves) {
+        const double at_once = D > 128 || waves == 8 ? 256.0 : 512.0, all = pre.groups + own.groups;
+        auto us = [&](const Part &x) { return x.bytes == 0.0 && all > 256.0 ? x.beside : x.alone; };
+        const double own_us = us(own), pre_us = us(pre);
+        // what split keys draw from memory, beside the time that row tiles hold the CUs
+        const double bytes = pre.bytes + own.bytes, rate = 5.5e6 * std::min(1.0, 0.6 + 0.4 * all / 256.0);
+        const double memory = bytes == 0.0 ? 0.0
+                                           : 5.0 + bytes / rate + 3.0 * ((pre.bytes > 0.0 ? pre.groups : 0.0) + (own.bytes > 0.0 ? own.groups : 0.0)) / 512.0 +
+                                                 (pre.groups > 0.0 && pre.bytes == 0.0 ? pre.groups * pre_us / at_once : 0.0);
+        if (pre.groups == 0.0) return std::max(memory, std::ceil(own.groups / at_once) * (own.bytes == 0.0 ? own_us : 0.0) + (own.bytes == 0.0 ? 0.0 : own_us));
+        // the prefix's whole rounds, the rest of it with own ones beside it, then the others wherever one ends first
+        const double before = std::floor(pre.groups / at_once) * pre_us, left = std::fmod(pre.groups, at_once), beside = at_once - left;
+        const double end = before + (left > 0.0 ? pre_us : 0.0), rest = own.groups - beside;
+        if (rest <= 0.0) return std::max({memory, end, before + own_us});
+        return std::max({memory, end, std::min(before + own_us * (1.0 + std::ceil(rest / beside)), end + own_us * std::ceil(rest / at_once))});
+    };
+    auto join = [&](int slots) { return slots > 1 ? 4.0 + (double)B * H * n_q * slots * D * 8 / 5e6 : 0.0; };
+    static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 28, 32, 48, 64, 96, 128};
     static_assert(128 <= ATTN_MAX_SLOTS / 2, "a prefix's splits and the batches' own");
     const int wide = D <= 128 ? 8 : 4;
     p.own_rows = rows > 32;
     p.pre_rows = t.kp && B * rows > 32;
-    double best = 0.0;
-    auto join = [&](int slots) { return slots > 1 ? 4.0 + (double)B * H * n_q * slots * D * 8 / 8e6 : 0.0; };
-    auto take = [&](int waves, int own, const Part &o, int pre, const Part &r) {
-        const double us = std::max({o.longest, r.longest, o.all + r.all}) + join(own + pre);
-        if (p.slots != 0 && us >= best) return;
-        best = us;
-        p.waves = waves;
-        p.own_splits = own;
-        p.own_tiles = o.tiles;
-        p.pre_splits = pre;
-        p.pre_tiles = r.tiles;
-        p.slots = own + pre;
-    };
     const int64_t n_kv = t.k.ne[1], n_pre = t.kp ? t.kp->ne[1] : 0;
-    // (two sets of row tiles gain by the wide workgroups; beside a memory-bound part two smaller ones do)
-    for (int waves = t.kp && p.own_rows ? wide : 4; waves <= (t.kp && !p.own_rows ? 4 : wide); waves += 4)
+    double best = 0.0;
+    // (row tiles may gain by the wide workgroups; split keys do not, and beside them two smaller ones do better)
+    for (int waves = t.kp && p.own_rows ? wide : 4; waves <= (p.own_rows ? wide : 4); waves += 4)
         for (int so : SPLITS) {
-            if (so > 1 && (so - 1) * 32 >= n_kv) break;
-            const Part o = part(rows, B * Hk, n_kv, p.own_rows, waves, so, !t.kp);
-            if (!t.kp) {
-                take(waves, so, o, 0, Part{0.0, 0.0, 0});
-                continue;
-            }
+            if (so > 1 && ((so - 1) * 32 >= n_kv || (t.kp && so > 4))) break;
+            const Part own = part(rows, B * Hk, n_kv, p.own_rows, waves, so);
             for (int sp : SPLITS) {
                 if (sp > 1 && (sp - 1) * 32 >= n_pre) break;
-                take(waves, so, o, sp, part(B * rows, Hk, n_pre, p.pre_rows, waves, sp, false));
+                const Part pre = t.kp ? part(B * rows, Hk, n_pre, p.pre_rows, waves, sp) : Part{};
+                const int slots = t.kp ? so + sp : so;
+                const double us = launch(pre, own, waves) + join(slots);
+                if (p.slots != 0 && us >= best) continue;
+                best = us;
+                p.waves = waves;
+                p.own_splits = so;
+                p.own_tiles = own.tiles;
+                p.pre_splits = t.kp ? sp : 0;
+                p.pre_tiles = pre.tiles;
+                p.slots = slots;
             }
         }
     return p;

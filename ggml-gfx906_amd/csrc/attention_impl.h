@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // wants from that lane once the keys are taken in the order the MFMA returned them: the weights never
 // leave the registers. Tiles come by LDS DMA, one tile ahead.
 //   BY_ROWS: 4 or 8 waves of 32 rows each share tiles of KT keys (prompts, shared prefixes)
-//   else:    4 or 8 waves share 32 rows and take tiles of 32 keys in turn, joined at the end (tokens)
+//   else:    the waves share 32 rows and take tiles of 32 keys in turn, joined at the end (tokens)
 // 16-byte pieces of a tile's rows are permuted (swz_k, swz_v) so that neither read meets an LDS bank
 // twice; the DMA writes LDS in order, so the permutation is in the addresses it reads from.
 //
@@ -612,8 +612,20 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 #pragma unroll
             for (int r = 0; r < KT / 8; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[r][e] = 8 * r + e < left ? mp[8 * r + e] : (_Float16)0.0f;
+                for (int e = 0; e < 4; ++e) w[r][e] = 8 * r + e < left ? mp[8 * r + e] : (_Float16)-INFINITY;
         }
+    };
+
+    // whether the mask hides the tile from all of the wave's rows
+    auto hidden = [&](const f16x4 (&w)[KT / 8]) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        uint32_t other = 0;
+#pragma unroll
+        for (int r = 0; r < KT / 8; ++r) {
+            const u32x2 v = __builtin_bit_cast(u32x2, w[r]);
+            other |= (v[0] ^ 0xfc00fc00u) | (v[1] ^ 0xfc00fc00u);
+        }
+        return __all(other == 0);
     };
 
     // LDS reads run AHEAD operands ahead of the MFMAs that take them: left to itself the compiler, short of
@@ -750,7 +762,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 load_v(j + KT, next + BYTES);
                 if (masked) fetch(j + KT, ahead);
             }
-            if (j < seen_most) {
+            if (j < seen_most && !(masked && hidden(w))) {
                 // (a wave that feeds the matrix cores goes before one that forms weights)
                 __builtin_amdgcn_s_setprio(1);
                 products(now);
@@ -780,17 +792,14 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 }
                 if (j + STEP < j_end) fetch(j + STEP, ahead);
             }
-            products(stage0);
+            const bool idle = masked && hidden(w);
+            if (!idle) products(stage0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (j + STEP < j_end) {
-                load_k(j + STEP, stage0);
-                weights(j, w);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory");   // the values
-            } else {
-                weights(j, w);
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            values(stage0 + BYTES);
+            if (j + STEP < j_end) load_k(j + STEP, stage0);
+            if (!idle) weights(j, w);
+            if (j + STEP < j_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory");   // the values
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (!idle) values(stage0 + BYTES);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (j + STEP < j_end) load_v(j + STEP, stage0 + BYTES);
         }
@@ -875,10 +884,8 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
         else if (general) ATTN_CASE(4, 0, false, true);
         else ATTN_CASE(4, 0, false, false);
     } else {
-        if (pl.own_rows && general) ATTN_CASE(WIDE, 0, true, true);
-        else if (pl.own_rows) ATTN_CASE(WIDE, 0, true, false);
-        else if (general) ATTN_CASE(WIDE, 0, false, true);
-        else ATTN_CASE(WIDE, 0, false, false);
+        if (general) ATTN_CASE(WIDE, 0, true, true);
+        else ATTN_CASE(WIDE, 0, true, false);
     }
 #undef ATTN_CASE
     if (pl.slots > 1) {

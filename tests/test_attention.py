@@ -200,6 +200,23 @@ def test_masks(kv, io, n, m, bias, planes):
 
 @gpu
 @pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 6, 300])
+def test_masks_that_hide_whole_tiles(kv, io, n):
+    """several sequences in one cache: each row sees a stretch of it somewhere, and what lies between is hidden
+    from every row (and NaN)"""
+    m = 1100
+    q, k, v = operands(1, n, m, 8, 2, 64, kv, io, seed=2)
+    w = torch.full((1, 1, n, m), -INF, dtype=torch.float16, device="cuda")
+    for i in range(n):
+        first = 700 if i % 3 == 0 else 100 + i % 7
+        w[0, 0, i, first : first + 60 + i % 50] = 0.25 * (i % 4)
+    dead = (w == -INF).all(2)[0, 0]
+    k[:, dead], v[:, dead] = NAN, NAN
+    near(call(q, k, v, 0.125, mask=w), formula(q, k, v, 0.125, full(1, m), mask=w))
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
 @pytest.mark.parametrize("n", [1, 4, 40, 140])
 def test_unseen_keys_may_hold_anything(kv, io, n):
     """NaN and infinities in keys that the mask hides from some rows or the causal rule hides from the first:
