@@ -298,11 +298,13 @@ template <typename TK, typename TQ, int DP, bool PREFIX>
 __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DP / 32], float m, float l, int row,
                                            bool row_ok, int bh, int split, int j_begin, int j_end) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    bool bad = l != l;
+    // (a sum of infinities of both signs is NaN too: such a row is done again for nothing, to the same result)
+    float all = l;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) bad |= o[d][r] != o[d][r];
+        for (int d = 0; d < DP / 32; ++d) all += o[d][r];
+    const bool bad = all != all;
     const uint64_t votes = __ballot(bad && row_ok);
     uint32_t again = (uint32_t)votes | (uint32_t)(votes >> 32);
     if (row_ok && !(again >> (lane & 31) & 1)) {
@@ -318,8 +320,8 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
+                if (32 * d + 8 * r4 >= a.D) continue;   // (D is a multiple of 8)
                 const int at = 32 * d + 8 * r4 + 4 * h;
-                if (at >= a.D) continue;
                 const f32x4 x = f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]} * f;
                 if (p.part_o) *reinterpret_cast<f32x4 *>(po + at) = x;
                 else store4<TQ>(out + at, x);
@@ -332,65 +334,66 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
     }
 }
 
-// 32 rows that the waves hold parts of, each in its stretch of LDS (values [row][DP], then the maxima and
-// the sums): two threads of each wave a row
+// the place of piece c (four values) of row r in a wave's stretch of LDS: permuted by the row, against bank conflicts
+template <int DP> __device__ __forceinline__ int piece_at(int r, int c) { return (r * (DP / 4) + (c ^ (r & (DP / 4 - 1)))) * 16; }
+
+// up to 32 rows that the waves hold parts of, each in its stretch of LDS (pieces of the rows, then the maxima and
+// the sums): a thread a piece, so that a token's few rows are spread over all threads
 template <typename TK, typename TQ, int DP, int WAVES, bool PREFIX>
 __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p, const char *lds, int stretch, int tops, int row0, int bh,
                                            int split, int j_begin, int j_end) {
-    constexpr int TPR = WAVES * 2, N = DP / TPR;
-    const int r = threadIdx.x / TPR, d0 = threadIdx.x % TPR * N, row = row0 + r;
-    const bool ok = row < p.rows;
-    float m = -INFINITY, l = 0.0f, f[WAVES];
-    f32x4 x[N / 4];
+    constexpr int PIECES = DP / 4, AT_ONCE = WAVES * 64 / PIECES;   // of a row; rows
+    const int lane = threadIdx.x & 63, c = threadIdx.x % PIECES, n = min(32, p.rows - row0);
+    for (int r0 = 0; r0 < n; r0 += AT_ONCE) {
+        const int r = r0 + threadIdx.x / PIECES, row = row0 + min(r, n - 1);
+        const bool ok = r < n;
+        float m = -INFINITY, l = 0.0f;
+        f32x4 x{};
+        if (ok) {
+            float mw[WAVES];
+            f32x4 xw[WAVES];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, reinterpret_cast<const float *>(lds + w * stretch + tops)[r]);
+            for (int w = 0; w < WAVES; ++w) {
+                mw[w] = reinterpret_cast<const float *>(lds + w * stretch + tops)[r];
+                xw[w] = *reinterpret_cast<const f32x4 *>(lds + w * stretch + piece_at<DP>(r, c));
+                m = fmaxf(m, mw[w]);
+            }
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const float *ml = reinterpret_cast<const float *>(lds + w * stretch + tops);
-        f[w] = m == -INFINITY ? 1.0f : exp2f(ml[r] - m);
-        l += ml[32 + r] * f[w];
-    }
-#pragma unroll
-    for (int e = 0; e < N / 4; ++e) {
-        x[e] = f32x4{};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) x[e] += *reinterpret_cast<const f32x4 *>(lds + w * stretch + (r * DP + d0 + 4 * e) * 4) * f[w];
-    }
-    bool bad = l != l;
-#pragma unroll
-    for (int e = 0; e < N / 4; ++e)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) bad |= x[e][c] != x[e][c];
-    // a row's threads are neighbours in one wave: any of their votes counts
-    uint64_t again = __ballot(bad && ok);
-#pragma unroll
-    for (int sft = 1; sft < TPR; sft <<= 1) again |= again >> sft;
-    uint64_t firsts = 0;
-#pragma unroll
-    for (int t = 0; t < 64; t += TPR) firsts |= 1ull << t;
-    again &= firsts;
-    const int lane = threadIdx.x & 63;
-    if (ok && !(again >> (lane / TPR * TPR) & 1)) {
-        const RowOut w = row_out<PREFIX>(a, p, row, bh, split);
-        if (p.part_o && d0 == 0) {
-            p.part_ml[2 * w.slot] = m;
-            p.part_ml[2 * w.slot + 1] = l;
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = m == -INFINITY ? 1.0f : exp2f(mw[w] - m);
+                l += reinterpret_cast<const float *>(lds + w * stretch + tops)[32 + r] * f;
+                x += xw[w] * f;
+            }
         }
-        const float s = p.part_o ? 1.0f : finish(a, w.head, m, l);
-        float *po = p.part_o + w.slot * a.D;
-        TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
+        // a row's threads are neighbours in one wave: any of their votes counts
+        const float all = (x[0] + x[1]) + (x[2] + x[3]) + l;
+        uint64_t again = __ballot(ok && all != all);
+        if (again) {
 #pragma unroll
-        for (int e = 0; e < N / 4; ++e) {
-            const int at = d0 + 4 * e;
-            if (at >= a.D) continue;
-            if (p.part_o) *reinterpret_cast<f32x4 *>(po + at) = x[e];
-            else store4<TQ>(out + at, x[e] * s);
+            for (int sft = 1; sft < PIECES; sft <<= 1) again |= again >> sft;
+            uint64_t firsts = 0;
+#pragma unroll
+            for (int t = 0; t < 64; t += PIECES) firsts |= 1ull << t;
+            again &= firsts;
         }
-    }
-    while (again) {
-        const int at = __builtin_ctzll(again);
-        again &= again - 1;
-        redo_row<TK, TQ, PREFIX>(a, p, __builtin_amdgcn_readlane(row, at), bh, split, j_begin, j_end);
+        if (ok && 4 * c < a.D && !(again >> (lane / PIECES * PIECES) & 1)) {
+            const RowOut w = row_out<PREFIX>(a, p, row, bh, split);
+            if (p.part_o) {
+                if (c == 0) {
+                    p.part_ml[2 * w.slot] = m;
+                    p.part_ml[2 * w.slot + 1] = l;
+                }
+                *reinterpret_cast<f32x4 *>(p.part_o + w.slot * a.D + 4 * c) = x;
+            } else {
+                TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
+                store4<TQ>(out + 4 * c, x * finish(a, w.head, m, l));
+            }
+        }
+        while (again) {
+            const int at = __builtin_ctzll(again);
+            again &= again - 1;
+            redo_row<TK, TQ, PREFIX>(a, p, __builtin_amdgcn_readlane(row, at), bh, split, j_begin, j_end);
+        }
     }
 }
 
@@ -476,6 +479,30 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int i = PREFIX ? bi % a.n_q : bi, b = PREFIX ? bi / a.n_q : pb;
     const int head = hk * G + g;
 
+    // queries: lane (row, h) holds values 16 t + 8 h .. + 7 of its row. They are asked for before anything that waits for
+    // the batch's length, and the first tile's DMA follows; one wait covers both (the compiler, which knows of
+    // the queries only, would otherwise wait inside the loop, and there for the tile ahead too)
+    x8 qf[NT], ql[SPLIT ? NT : 1];
+    f32x4 qx[SPLIT ? 2 * NT : 1];
+    {
+        const char *qr = a.q + i * a.q_i + head * a.q_h + b * a.q_b;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int d = 16 * t + 8 * h;
+            if constexpr (SPLIT) {
+                qx[2 * t] = qx[2 * t + 1] = f32x4{};
+                if (d < a.D) {
+                    qx[2 * t] = *reinterpret_cast<const f32x4 *>(qr + 4 * d);
+                    qx[2 * t + 1] = *reinterpret_cast<const f32x4 *>(qr + 4 * d + 16);
+                }
+            } else {
+                x8 z{};
+                qf[t] = d < a.D ? *reinterpret_cast<const x8 *>(qr + 2 * d) : z;
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
     // keys of this split, and how many of them the lane's row sees
     const int n = PREFIX ? a.n_prefix : own_len(a, b);
     int end = n;                                    // of the workgroup's rows
@@ -510,6 +537,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     // the tile at key j into `dst`, this wave's (BY_ROWS: the workgroup's) LDS
     const int ltid = BY_ROWS ? tid : lane, lrow = ltid / CPR, place = ltid % CPR;
     char *stage0 = lds + (BY_ROWS ? 0 : wave * T::STRETCH);
+    const uint32_t k_row = lrow * (uint32_t)k_j, v_row = lrow * (uint32_t)v_j;
     auto load = [&](const char *base, int64_t stride, int j, char *dst, auto swz) {
         char *to = dst + (BY_ROWS ? wave * 1024 : 0);
         const i32x4 buf = buffer_at(base + j * stride);
@@ -528,57 +556,33 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     auto load_k = [&](int j, char *dst) { load(kb, k_j, j, dst, [](int r) { return swz_k<DP>(r); }); };
     auto load_v = [&](int j, char *dst) { load(vb, v_j, j, dst, [](int r) { return swz_v<DP>(r); }); };
 
-    // the first tile's DMA, then the queries, then one wait for both: the compiler, which knows of the
-    // latter only, would otherwise wait inside the loop, and there for the tile ahead too
     const int j0 = BY_ROWS ? j_begin : j_begin + wave * 32;
     if (j0 < j_end) {
         load_k(j0, stage0);
         load_v(j0, stage0 + BYTES);
     }
 
-    // queries: lane (row, h) holds values 16 t + 8 h .. + 7 of its row
-    x8 qf[NT], ql[SPLIT ? NT : 1];
     float c = a.scale;
-    {
-        const char *qr = a.q + i * a.q_i + head * a.q_h + b * a.q_b;
-        if constexpr (SPLIT) {
-            float v[NT][8], top = 0.0f;
+    if constexpr (SPLIT) {
+        float top = 0.0f;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int d = 16 * t + 8 * h;
-                f32x4 x0{}, x1{};
-                if (d < a.D) {
-                    x0 = *reinterpret_cast<const f32x4 *>(qr + 4 * d);
-                    x1 = *reinterpret_cast<const f32x4 *>(qr + 4 * d + 16);
-                }
+        for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[t][e] = x0[e];
-                    v[t][4 + e] = x1[e];
-                    top = fmaxf(top, fmaxf(fabsf(x0[e]), fabsf(x1[e])));
-                }
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(qx[t][e]));
+        top = fmaxf(top, swap32_f(top));
+        // 2^-e * q below 1: no f16 overflows, and the second term keeps its bits
+        int e2 = 0;
+        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = ldexpf(qx[2 * t + e / 4][e % 4], -e2);
+                const _Float16 hi = (_Float16)x;
+                qf[t][e] = hi;
+                ql[t][e] = (_Float16)(x - (float)hi);
             }
-            top = fmaxf(top, swap32_f(top));
-            // 2^-e * q below 1: no f16 overflows, and the second term keeps its bits
-            int e2 = 0;
-            if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float x = ldexpf(v[t][e], -e2);
-                    const _Float16 hi = (_Float16)x;
-                    qf[t][e] = hi;
-                    ql[t][e] = (_Float16)(x - (float)hi);
-                }
-            c = ldexpf(c, e2);
-        } else {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                x8 z{};
-                qf[t] = 16 * t + 8 * h < a.D ? *reinterpret_cast<const x8 *>(qr + 2 * (16 * t + 8 * h)) : z;
-            }
-        }
+        c = ldexpf(c, e2);
     }
     const bool capped = KIND != OWN && a.cap != 0.0f;
     const float c_cap = capped ? c / a.cap : 0.0f, cap2 = a.cap * LOG2E;
@@ -651,6 +655,33 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, PER * AHEAD, 0);
+    };
+    // the same with the next tile's DMA (a whole one, into `to`) dealt out among the MFMAs: issued in a row it holds a
+    // wave up for 1000 cycles, a quarter of a tile's time
+    auto products_and_load = [&](const char *kt, int j, char *to) {
+        constexpr int NQK = KT / 32 * NT, EVERY = NQK / (2 * ROUNDS) > 0 ? NQK / (2 * ROUNDS) : 1;
+        static_assert(!BY_ROWS || 2 * ROUNDS * EVERY <= NQK, "every DMA has its step");
+        const int krow = lane & 31, ksw = swz_k<DP>(krow);
+        const i32x4 kbuf = buffer_at(kb + j * k_j), vbuf = buffer_at(vb + j * v_j);
+        auto read = [&](int n) { return *reinterpret_cast<const x8 *>(kt + (n / NT * 32 + krow) * DP * 2 + (((2 * (n % NT) + h) ^ ksw) * 16)); };
+        x8 kf[AHEAD];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) kf[n] = read(n);
+#pragma unroll
+        for (int n = 0; n < NQK; ++n) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x16 from = n % NT == 0 ? f32x16{} : s[n / NT];
+            s[n / NT] = mma(kf[n % AHEAD], qf[n % NT], from);
+            if constexpr (SPLIT) s[n / NT] = mma(kf[n % AHEAD], ql[n % NT], s[n / NT]);
+            if (n + AHEAD < NQK) kf[n % AHEAD] = read(n + AHEAD);
+            if (n % EVERY == 0 && n / EVERY < 2 * ROUNDS) {
+                const int u = n / EVERY / 2, r = u * RPI + lrow;
+                char *at = to + wave * 1024 + u * T::LOADERS * 16;
+                if (n / EVERY % 2 == 0) dma16(kbuf, at, k_row + piece_off(place, swz_k<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)k_j);
+                else dma16(vbuf, at + BYTES, v_row + piece_off(place, swz_v<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)v_j);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
     // the weights of the tile's keys from their products: s[u][r] belongs to key j + 32 u + 8 (r / 4) + 4 h +
     // r % 4, f times it is the score in units of log 2
@@ -757,15 +788,18 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                     asm volatile("" : "+v"(w[r]));
                 }
             }
-            if (j + KT < j_end) {
+            // (8 waves have half the DMA each, and lose 3 % by dealing it out)
+            const bool mine = j < seen_most && !(masked && hidden(w)), among = WAVES == 4 && mine && j + 2 * KT <= j_end;
+            if (j + KT < j_end && !among) {
                 load_k(j + KT, next);
                 load_v(j + KT, next + BYTES);
-                if (masked) fetch(j + KT, ahead);
             }
-            if (j < seen_most && !(masked && hidden(w))) {
+            if (masked && j + KT < j_end) fetch(j + KT, ahead);
+            if (mine) {
                 // (a wave that feeds the matrix cores goes before one that forms weights)
                 __builtin_amdgcn_s_setprio(1);
-                products(now);
+                if (among) products_and_load(now, j + KT, next);
+                else products(now);
                 __builtin_amdgcn_s_setprio(0);
                 weights(j, w);
                 __builtin_amdgcn_s_setprio(1);
@@ -810,17 +844,18 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     if constexpr (!BY_ROWS) {
         // join the waves: each leaves its rows in its own stretch
         asm volatile("" ::: "memory");
-        float *po = reinterpret_cast<float *>(stage0), *pm = reinterpret_cast<float *>(stage0 + 2 * BYTES);
+        if (row_ok) {
+            float *pm = reinterpret_cast<float *>(stage0 + 2 * BYTES);
 #pragma unroll
-        for (int d = 0; d < NB; ++d)
+            for (int d = 0; d < NB; ++d)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const f32x4 x = {o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
-                *reinterpret_cast<f32x4 *>(po + (lane & 31) * DP + 32 * d + 8 * r4 + 4 * h) = x;
+                for (int r4 = 0; r4 < 4; ++r4)
+                    *reinterpret_cast<f32x4 *>(stage0 + piece_at<DP>(lane & 31, 8 * d + 2 * r4 + h)) =
+                        f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+            if (h == 0) {
+                pm[lane] = me;
+                pm[32 + lane] = l;
             }
-        if (h == 0) {
-            pm[lane] = me;
-            pm[32 + lane] = l;
         }
         __syncthreads();
         join_waves<TK, TQ, DP, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
@@ -889,11 +924,11 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     }
 #undef ATTN_CASE
     if (pl.slots > 1) {
-        // a row's splits side by side (8 of them with 128 values a row, at most 8 a thread then) where rows are
-        // few; one group of threads a row where a row has a few splits or its rows fill the CUs by themselves
+        // a workgroup a row, its splits side by side, where rows are few; one group of threads a row where it has a
+        // few splits and the rows fill the CUs by themselves (6400 rows of 4 splits: 11.6 us and 5.7)
         const int64_t rows = (int64_t)a.B * a.H * a.n_q;
         constexpr int ALL = 1024 / DP;
-        if (pl.slots <= 2 || (pl.slots <= 8 && rows >= 8192)) {
+        if (pl.slots <= 2 || (pl.slots <= 8 && rows >= 2048)) {
             const unsigned grid = (unsigned)((rows * (DP / 4) + 255) / 256);
             hipLaunchKernelGGL((attn_join_kernel<TQ, DP, 1>), dim3(grid), dim3(256), 0, st, a, own);
         } else {
