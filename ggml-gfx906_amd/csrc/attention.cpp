@@ -212,7 +212,9 @@ int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t 
     a.o = static_cast<char *>(d.data);
     a.o_h = (int64_t)d.nb[1]; a.o_i = (int64_t)d.nb[2]; a.o_b = (int64_t)d.nb[3];
     a.D = (int)q.ne[0]; a.n_q = (int)q.ne[1]; a.n_kv = (int)k.ne[1];
-    a.H = (int)q.ne[2]; a.Hk = (int)k.ne[2]; a.B = (int)q.ne[3]; a.kv_b = (int)(q.ne[3] / k.ne[3]);
+    a.H = (int)q.ne[2]; a.Hk = (int)k.ne[2]; a.B = (int)q.ne[3];
+    a.by_G = Div((uint32_t)(a.H / a.Hk)); a.by_Hk = Div((uint32_t)a.Hk); a.by_n_q = Div((uint32_t)a.n_q);
+    a.by_kv_b = Div((uint32_t)(q.ne[3] / k.ne[3]));
     a.causal = p.causal;
     a.scale = p.scale;
     a.cap = p.logit_softcap;

@@ -6,6 +6,17 @@
 
 namespace mi355x {
 
+// n / d for 0 <= n < 2^31: the divisors are the same for a whole launch, a division takes some 40 instructions
+struct Div {
+    uint32_t d, mul, shift;
+    __host__ __device__ Div(uint32_t by = 1) : d(by), shift(0) {
+        while ((1ull << shift) < d) ++shift;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+    __device__ __forceinline__ int rest(int n) const { return n - of(n) * (int)d; }
+};
+
 struct AttnArgs {
     const char *q; int64_t q_i, q_h, q_b;
     const char *k; int64_t k_j, k_h, k_b;
@@ -18,7 +29,8 @@ struct AttnArgs {
     const float *sinks;
     const char *len; int64_t len_b;                  // i32 [batch], or nullptr: n_kv
     char *o; int64_t o_i, o_h, o_b;
-    int D, n_q, n_kv, n_prefix, H, Hk, B, kv_b;      // kv_b: batches that share one cache
+    int D, n_q, n_kv, n_prefix, H, Hk, B;
+    Div by_G, by_Hk, by_n_q, by_kv_b;                // G = H / Hk heads a key head; kv_b: batches that share one cache
     int causal;
     float scale, cap;                                // cap = 0: none
     int bias_heads;                                  // slopes: 0 = none, else the power of two of heads

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
     __shared__ RowState part[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int hk = h / (a.H / a.Hk), bk = b / a.kv_b;
+    const int hk = a.by_G.of(h), bk = a.by_kv_b.of(b);
     float q[4];
     const TQ *qr = reinterpret_cast<const TQ *>(a.q + i * a.q_i + h * a.q_h + b * a.q_b);
 #pragma unroll
@@ -177,26 +177,39 @@ template <int DP> __device__ __forceinline__ int swz_v(int r) { return DP == 64 
 // which keys and rows some of a launch's workgroups work on
 struct AttnPart {
     float *part_o, *part_ml;   // partial results, or nullptr: the call's result
-    int slot0, n_split;        // these splits among
+    int slot0;                 // these splits among
     int slots;                 // all partial results of a row
-    int n_bh;                  // (batch,) key / value head problems
+    Div by_split, by_bh;       // splits; (batch,) key / value head problems
     int rows, row_tiles;       // of each
     int blocks;
 };
 
-// 16 bytes per lane from base + voff + soff into LDS at dst + 16 * lane (dst, soff wave-uniform). Written out
-// because the compiler, which can not tell the stages apart, makes every LDS read wait for each DMA that it
-// knows of; the kernel waits itself. No result registers; the address registers are read at issue; m0 is
-// a reserved register, which the compiler sets right before an own use (these kernels have none). The nops are the wait states from a scalar's write by a vector instruction and from m0's to their use.
+// LDS DMA: 16 bytes per lane from the buffer into LDS, the wave's 1 KiB at dst + 1024 * u. Written out because the
+// compiler, which can not tell the stages apart, makes every LDS read wait for each DMA that it knows of; the
+// kernel waits itself. No result registers; the address registers are read at issue; m0, the LDS address, is a
+// reserved register, which the compiler sets right before an own use (these kernels have none). A change of m0
+// costs a DMA some 40 cycles, so four of them share one: the instruction's offset moves both addresses, and
+// the buffer begins DMA_BACK bytes early to give its share back. The nops are the wait states from a scalar's
+// write by a vector instruction and from m0's to their use.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ i32x4 buffer_at(const char *p) {   // a raw buffer of 2 GiB
-    const uint64_t at = (uint64_t)(uintptr_t)p;
+constexpr int DMA_BACK = 4096;
+__device__ __forceinline__ i32x4 buffer_at(const char *p) {   // a raw buffer of 2 GiB, from DMA_BACK bytes before p
+    const uint64_t at = (uint64_t)(uintptr_t)p - DMA_BACK;
     return i32x4{(int)__builtin_amdgcn_readfirstlane((uint32_t)at), (int)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32) & 0xffff), 0x7fffffff, 0x00020000};
 }
-__device__ __forceinline__ void dma16(i32x4 r, const char *dst, uint32_t voff, uint32_t soff) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_const)dst);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :: "s"(at), "v"(voff), "s"(r), "s"(soff) : "memory");
+// number u of a wave's DMAs in a row (dst: of the first), from byte voff (the lane's) + soff behind the buffer's p
+__device__ __forceinline__ void dma16(int u, i32x4 buf, const char *dst, uint32_t voff, uint32_t soff) {
+    const uint32_t s = soff + DMA_BACK - u % 4 * 1024;
+    switch (u % 4) {
+        case 0: {
+            const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_const)dst + (uint32_t)u * 1024);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(voff), "s"(buf), "s"(s) : "memory");
+            break;
+        }
+        case 1: asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:0x400 lds" ::"v"(voff), "s"(buf), "s"(s) : "memory"); break;
+        case 2: asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:0x800 lds" ::"v"(voff), "s"(buf), "s"(s) : "memory"); break;
+        default: asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen offset:0xc00 lds" ::"v"(voff), "s"(buf), "s"(s) : "memory");
+    }
 }
 
 template <typename TK, typename TQ, int DP, int WAVES, bool BY_ROWS>
@@ -204,9 +217,8 @@ struct AttnTile {
     static constexpr bool SPLIT = sizeof(TQ) == 4;
     static constexpr int KT = BY_ROWS && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int CPR = DP / 8;                          // 16-byte pieces of a row
-    static constexpr int LOADERS = BY_ROWS ? WAVES * 64 : 64;   // threads that load a tile together
-    static constexpr int RPI = LOADERS / CPR;                   // rows of one DMA round
-    static constexpr int ROUNDS = KT / RPI;
+    static constexpr int RPD = 64 / CPR;                        // rows of a DMA
+    static constexpr int ROUNDS = KT / RPD / (BY_ROWS ? WAVES : 1);   // a wave's DMAs of a tile of keys, or of values
     static constexpr int BYTES = KT * DP * 2;                   // of a tile of keys, and of values
     // BY_ROWS: two stages of keys and values; else one of each per wave, whose 32 rows also fit it as f32,
     // and those rows' maxima and sums
@@ -223,10 +235,10 @@ struct RowOut {
 };
 template <bool PREFIX>
 __device__ __forceinline__ RowOut row_out(const AttnArgs &a, const AttnPart &p, int row, int bh, int split) {
-    const int G = a.H / a.Hk, hk = bh % a.Hk, g = row % G, bi = row / G;
+    const int G = (int)a.by_G.d, pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk, bi = a.by_G.of(row), g = row - bi * G;
     RowOut r;
-    r.i = PREFIX ? bi % a.n_q : bi;
-    r.b = PREFIX ? bi / a.n_q : bh / a.Hk;
+    r.b = PREFIX ? a.by_n_q.of(bi) : pb;
+    r.i = PREFIX ? bi - r.b * a.n_q : bi;
     r.head = hk * G + g;
     r.slot = (((int64_t)r.b * a.Hk + hk) * a.n_q * G + r.i * G + g) * p.slots + p.slot0 + split;
     return r;
@@ -252,7 +264,7 @@ template <typename TK, typename TQ, bool PREFIX>
 __device__ void redo_row(const AttnArgs &a, const AttnPart &p, int row, int bh, int split, int j_begin, int j_end) {
     const int lane = threadIdx.x & 63;
     const RowOut w = row_out<PREFIX>(a, p, row, bh, split);
-    const int hk = bh % a.Hk, bk = PREFIX ? 0 : (bh / a.Hk) / a.kv_b;
+    const int pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk, bk = PREFIX ? 0 : a.by_kv_b.of(pb);
     float q[4];
     const TQ *qr = reinterpret_cast<const TQ *>(a.q + w.i * a.q_i + w.head * a.q_h + w.b * a.q_b);
 #pragma unroll
@@ -404,10 +416,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a, const 
     constexpr int LPR = DP / 4, TPR = LPR * GROUPS, ROWS = 256 / TPR;
     __shared__ f32x4 part[ROWS][GROUPS == 1 ? 1 : GROUPS][GROUPS == 1 ? 1 : LPR];
     const int tid = threadIdx.x, row = tid / TPR, grp = tid % TPR / LPR, d = tid % LPR * 4;
-    const int64_t rows = (int64_t)a.B * a.H * a.n_q, rr = min((int64_t)blockIdx.x * ROWS + row, rows - 1);
-    const int G = a.H / a.Hk, per = a.n_q * G;
-    const int r = (int)(rr % per), hk = (int)(rr / per % a.Hk), b = (int)(rr / per / a.Hk), i = r / G, head = hk * G + r % G;
-    const float *po = p.part_o + rr * p.slots * a.D + d, *ml = p.part_ml + 2 * rr * p.slots;
+    // rows lie by batch, key head, query, head of the group
+    const int rows = a.B * a.H * a.n_q, rr = min((int)blockIdx.x * ROWS + row, rows - 1);
+    const int G = (int)a.by_G.d, ri = a.by_G.of(rr), bhk = a.by_n_q.of(ri), b = a.by_Hk.of(bhk), i = ri - bhk * a.n_q;
+    const int head = (bhk - b * a.Hk) * G + rr - ri * G;
+    const float *po = p.part_o + (int64_t)rr * p.slots * a.D + d, *ml = p.part_ml + (int64_t)2 * rr * p.slots;
     const bool has = d < a.D;
     // (the first two of the thread's splits are on their way while the maximum forms)
     f32x4 x0{}, x1{};
@@ -444,7 +457,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a, const 
         part[row][grp][tid % LPR] = x;
         __syncthreads();
     }
-    if (grp != 0 || !has || (int64_t)blockIdx.x * ROWS + row >= rows) return;
+    if (grp != 0 || !has || (int)blockIdx.x * ROWS + row >= rows) return;
 #pragma unroll
     for (int g = 1; g < GROUPS; ++g) x += part[row][g][tid % LPR];   // (by the row's first group, in order)
     TQ *out = reinterpret_cast<TQ *>(a.o + i * a.o_i + head * a.o_h + b * a.o_b);
@@ -463,21 +476,19 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     using T = AttnTile<TK, TQ, DP, WAVES, BY_ROWS>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
-    constexpr int KT = T::KT, CPR = T::CPR, RPI = T::RPI, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DP / 16, NB = DP / 32;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    constexpr int KT = T::KT, CPR = T::CPR, RPD = T::RPD, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DP / 16, NB = DP / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     // problem, row tile (the last ones first: with a causal rule they see the most keys), split of the keys
-    const int bh = id % p.n_bh;
-    id /= p.n_bh;
-    const int split = id % p.n_split, tile = p.row_tiles - 1 - id / p.n_split;
-    const int G = a.H / a.Hk, hk = bh % a.Hk, pb = bh / a.Hk;
+    const int bh = p.by_bh.rest(id), at = p.by_bh.of(id), behind = p.by_split.of(at);
+    const int split = at - behind * (int)p.by_split.d, tile = p.row_tiles - 1 - behind;
+    const int G = (int)a.by_G.d, pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk;
 
     // this lane's row
     const int row0 = (BY_ROWS ? tile * WAVES + wave : tile) * 32;
     const int row = min(row0 + (lane & 31), p.rows - 1);
     const bool row_ok = row0 + (lane & 31) < p.rows;
-    const int g = row % G, bi = row / G;
-    const int i = PREFIX ? bi % a.n_q : bi, b = PREFIX ? bi / a.n_q : pb;
-    const int head = hk * G + g;
+    const int bi = a.by_G.of(row), head = hk * G + row - bi * G;
+    const int b = PREFIX ? a.by_n_q.of(bi) : pb, i = PREFIX ? bi - b * a.n_q : bi;
 
     // queries: lane (row, h) holds values 16 t + 8 h .. + 7 of its row. They are asked for before anything that waits for
     // the batch's length, and the first tile's DMA follows; one wait covers both (the compiler, which knows of
@@ -491,13 +502,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             const int d = 16 * t + 8 * h;
             if constexpr (SPLIT) {
                 qx[2 * t] = qx[2 * t + 1] = f32x4{};
-                if (d < a.D) {
+                if (d < a.D && row_ok) {
                     qx[2 * t] = *reinterpret_cast<const f32x4 *>(qr + 4 * d);
                     qx[2 * t + 1] = *reinterpret_cast<const f32x4 *>(qr + 4 * d + 16);
                 }
             } else {
                 x8 z{};
-                qf[t] = d < a.D ? *reinterpret_cast<const x8 *>(qr + 2 * d) : z;
+                qf[t] = d < a.D && row_ok ? *reinterpret_cast<const x8 *>(qr + 2 * d) : z;
             }
         }
     }
@@ -507,12 +518,12 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int n = PREFIX ? a.n_prefix : own_len(a, b);
     int end = n;                                    // of the workgroup's rows
     if (!PREFIX && a.causal) {
-        const int last = min((BY_ROWS ? (tile + 1) * WAVES : tile + 1) * 32 - 1, p.rows - 1) / G;
-        end = max(0, n - a.n_q + last + 1);
+        const int last = min((BY_ROWS ? (tile + 1) * WAVES : tile + 1) * 32 - 1, p.rows - 1);
+        end = max(0, n - a.n_q + a.by_G.of(last) + 1);
     }
     int j_begin = 0, j_end = end;
-    if (p.n_split > 1) {
-        const int per = ((end + p.n_split - 1) / p.n_split + T::STEP - 1) / T::STEP * T::STEP;
+    if (p.by_split.d > 1) {
+        const int per = (p.by_split.of(end + (int)p.by_split.d - 1) + T::STEP - 1) / T::STEP * T::STEP;
         j_begin = min(end, split * per);
         j_end = min(end, j_begin + per);
     }
@@ -530,31 +541,34 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         slope = fmaxf(slope_of(a, head) * LOG2E, 0x1p-100f);
     }
 
-    const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + (int64_t)(pb / a.kv_b) * a.k_b;
-    const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + (int64_t)(pb / a.kv_b) * a.v_b;
+    const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + (int64_t)a.by_kv_b.of(pb) * a.k_b;
+    const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + (int64_t)a.by_kv_b.of(pb) * a.v_b;
     const int64_t k_j = PREFIX ? a.kp_j : a.k_j, v_j = PREFIX ? a.vp_j : a.v_j;
 
     // the tile at key j into `dst`, this wave's (BY_ROWS: the workgroup's) LDS
-    const int ltid = BY_ROWS ? tid : lane, lrow = ltid / CPR, place = ltid % CPR;
+    // (its waves take ROUNDS pieces of RPD rows each)
+    const int lrow = lane / CPR, place = lane % CPR, first = BY_ROWS ? wave * ROUNDS : 0;
     char *stage0 = lds + (BY_ROWS ? 0 : wave * T::STRETCH);
     const uint32_t k_row = lrow * (uint32_t)k_j, v_row = lrow * (uint32_t)v_j;
-    auto load = [&](const char *base, int64_t stride, int j, char *dst, auto swz) {
-        char *to = dst + (BY_ROWS ? wave * 1024 : 0);
+    auto load = [&](const char *base, int64_t stride, uint32_t row0, int j, char *dst, auto swz) {
+        const char *to = dst + first * 1024;
         const i32x4 buf = buffer_at(base + j * stride);
         const uint32_t step = (uint32_t)stride;
         const int last = j_end - 1 - j;
         if (last >= KT - 1) {
 #pragma unroll
             for (int u = 0; u < ROUNDS; ++u)
-                dma16(buf, to + u * T::LOADERS * 16, lrow * step + piece_off(place, swz(u * RPI + lrow), a.D), (uint32_t)(u * RPI) * step);
+                dma16(u, buf, to, row0 + piece_off(place, swz((first + u) * RPD + lrow), a.D), (uint32_t)((first + u) * RPD) * step);
         } else {   // rows behind the keys: the last key again
 #pragma unroll
-            for (int u = 0; u < ROUNDS; ++u)
-                dma16(buf, to + u * T::LOADERS * 16, (uint32_t)min(u * RPI + lrow, last) * step + piece_off(place, swz(u * RPI + lrow), a.D), 0);
+            for (int u = 0; u < ROUNDS; ++u) {
+                const int r = (first + u) * RPD + lrow;
+                dma16(u, buf, to, (uint32_t)min(r, last) * step + piece_off(place, swz(r), a.D), 0);
+            }
         }
     };
-    auto load_k = [&](int j, char *dst) { load(kb, k_j, j, dst, [](int r) { return swz_k<DP>(r); }); };
-    auto load_v = [&](int j, char *dst) { load(vb, v_j, j, dst, [](int r) { return swz_v<DP>(r); }); };
+    auto load_k = [&](int j, char *dst) { load(kb, k_j, k_row, j, dst, [](int r) { return swz_k<DP>(r); }); };
+    auto load_v = [&](int j, char *dst) { load(vb, v_j, v_row, j, dst, [](int r) { return swz_v<DP>(r); }); };
 
     const int j0 = BY_ROWS ? j_begin : j_begin + wave * 32;
     if (j0 < j_end) {
@@ -675,10 +689,10 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             if constexpr (SPLIT) s[n / NT] = mma(kf[n % AHEAD], ql[n % NT], s[n / NT]);
             if (n + AHEAD < NQK) kf[n % AHEAD] = read(n + AHEAD);
             if (n % EVERY == 0 && n / EVERY < 2 * ROUNDS) {
-                const int u = n / EVERY / 2, r = u * RPI + lrow;
-                char *at = to + wave * 1024 + u * T::LOADERS * 16;
-                if (n / EVERY % 2 == 0) dma16(kbuf, at, k_row + piece_off(place, swz_k<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)k_j);
-                else dma16(vbuf, at + BYTES, v_row + piece_off(place, swz_v<DP>(r), a.D), (uint32_t)(u * RPI) * (uint32_t)v_j);
+                const int u = n / EVERY % ROUNDS, r = (first + u) * RPD + lrow;
+                const uint32_t rows = (uint32_t)((first + u) * RPD);
+                if (n / EVERY < ROUNDS) dma16(u, kbuf, to + first * 1024, k_row + piece_off(place, swz_k<DP>(r), a.D), rows * (uint32_t)k_j);
+                else dma16(u, vbuf, to + BYTES + first * 1024, v_row + piece_off(place, swz_v<DP>(r), a.D), rows * (uint32_t)v_j);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -883,7 +897,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attn_tile_kerne
 
 template <typename TK, typename TQ, int DP>
 static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
-    const int G = a.H / a.Hk;
+    const int G = (int)a.by_G.d;
     AttnPart own{}, pre{};
     own.slots = pl.slots;
     if (pl.slots > 1) {
@@ -892,18 +906,18 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     }
     pre = own;
     if (pl.pre_splits) {
-        pre.n_split = pl.pre_splits;
-        pre.n_bh = a.Hk;
+        pre.by_split = Div((uint32_t)pl.pre_splits);
+        pre.by_bh = Div((uint32_t)a.Hk);
         pre.rows = a.B * a.n_q * G;
         pre.row_tiles = pl.pre_tiles;
-        pre.blocks = pre.n_bh * pre.row_tiles * pre.n_split;
+        pre.blocks = a.Hk * pre.row_tiles * pl.pre_splits;
     }
     own.slot0 = pl.pre_splits;
-    own.n_split = pl.own_splits;
-    own.n_bh = a.B * a.Hk;
+    own.by_split = Div((uint32_t)pl.own_splits);
+    own.by_bh = Div((uint32_t)(a.B * a.Hk));
     own.rows = a.n_q * G;
     own.row_tiles = pl.own_tiles;
-    own.blocks = own.n_bh * own.row_tiles * own.n_split;
+    own.blocks = a.B * a.Hk * own.row_tiles * pl.own_splits;
     const bool general = a.mask != nullptr || a.cap != 0.0f;
     const dim3 grid((unsigned)(pre.blocks + own.blocks));
     constexpr int WIDE = DP == 256 ? 4 : 8;
