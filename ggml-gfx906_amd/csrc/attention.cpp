@@ -101,7 +101,7 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     // 110, 116; 64 sequences behind 8192 shared keys, 6 / 8 / 16 splits of them 54, 46, 53 / 65, 52, 58; 16 x 4 draft
     // tokens behind 32768, 24 / 28 / 32 splits 62, 58, 68 / 72, 72, 79.
     const int64_t D = t.q.ne[0], rows = n_q * G;
-    const double size = (D <= 64 ? 0.5 : 1.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
+    const double size = (D <= 64 ? 0.5 : D <= 96 ? 0.8 : 1.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
     struct Part { double groups, alone, beside, bytes; int tiles; };   // workgroups, us of each, bytes of split keys
     auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int s) {
         const int64_t per_tile = by_rows ? waves * 32 : 32, step = by_rows ? (D <= 128 ? 64 : 32) : 128;
@@ -225,11 +225,11 @@ int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t 
     }
     const AttnPlan pl = plan_attn(t);
     typedef hipError_t (*Launch)(const AttnArgs &, const AttnPlan &, void *, hipStream_t);
-    static const Launch launch[3][3] = {{attn_launch_f16_64, attn_launch_f16_128, attn_launch_f16_256},
-                                        {attn_launch_bf16_64, attn_launch_bf16_128, attn_launch_bf16_256},
-                                        {attn_launch_f32_64, attn_launch_f32_128, attn_launch_f32_256}};
+    static const Launch launch[3][4] = {{attn_launch_f16_64, attn_launch_f16_96, attn_launch_f16_128, attn_launch_f16_256},
+                                        {attn_launch_bf16_64, attn_launch_bf16_96, attn_launch_bf16_128, attn_launch_bf16_256},
+                                        {attn_launch_f32_64, attn_launch_f32_96, attn_launch_f32_128, attn_launch_f32_256}};
     const int type = q.type == T_F32 ? 2 : q.type == T_BF16 ? 1 : 0;
-    const hipError_t e = launch[type][a.D <= 64 ? 0 : a.D <= 128 ? 1 : 2](a, pl, work, st);
+    const hipError_t e = launch[type][a.D <= 64 ? 0 : a.D <= 96 ? 1 : a.D <= 128 ? 2 : 3](a, pl, work, st);
     return e == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
 }
 

@@ -51,12 +51,15 @@ struct AttnPlan {
 // to it; attention_kernels.hip). `work`: the partial results of pl.slots > 1
 #define ATTN_LAUNCH(NAME) hipError_t NAME(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st);
 ATTN_LAUNCH(attn_launch_f16_64)
+ATTN_LAUNCH(attn_launch_f16_96)
 ATTN_LAUNCH(attn_launch_f16_128)
 ATTN_LAUNCH(attn_launch_f16_256)
 ATTN_LAUNCH(attn_launch_bf16_64)
+ATTN_LAUNCH(attn_launch_bf16_96)
 ATTN_LAUNCH(attn_launch_bf16_128)
 ATTN_LAUNCH(attn_launch_bf16_256)
 ATTN_LAUNCH(attn_launch_f32_64)
+ATTN_LAUNCH(attn_launch_f32_96)
 ATTN_LAUNCH(attn_launch_f32_128)
 ATTN_LAUNCH(attn_launch_f32_256)
 #undef ATTN_LAUNCH

@@ -212,9 +212,14 @@ __device__ __forceinline__ void dma16(int u, i32x4 buf, const char *dst, uint32_
     }
 }
 
-template <typename TK, typename TQ, int DP, int WAVES, bool BY_ROWS>
+// DC: the head size that the products are formed for; DP: the next power of two, a row's place in LDS (what lies
+// behind the row is a copy of its last piece, and no product reads it beyond DC)
+constexpr int row_place(int DC) { return DC <= 64 ? 64 : DC <= 128 ? 128 : 256; }
+
+template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS>
 struct AttnTile {
     static constexpr bool SPLIT = sizeof(TQ) == 4;
+    static constexpr int DP = row_place(DC);
     static constexpr int KT = BY_ROWS && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int CPR = DP / 8;                          // 16-byte pieces of a row
     static constexpr int RPD = 64 / CPR;                        // rows of a DMA
@@ -306,8 +311,8 @@ template <> __device__ __forceinline__ void store4(__bf16 *p, f32x4 x) {
 }
 
 // a wave's 32 rows out of the accumulators: lane (row, h) holds values 32 d + 8 r4 + 4 h .. + 3
-template <typename TK, typename TQ, int DP, bool PREFIX>
-__device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DP / 32], float m, float l, int row,
+template <typename TK, typename TQ, int DC, bool PREFIX>
+__device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DC / 32], float m, float l, int row,
                                            bool row_ok, int bh, int split, int j_begin, int j_end) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     // (a sum of infinities of both signs is NaN too: such a row is done again for nothing, to the same result)
@@ -315,7 +320,7 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) all += o[d][r];
+        for (int d = 0; d < DC / 32; ++d) all += o[d][r];
     const bool bad = all != all;
     const uint64_t votes = __ballot(bad && row_ok);
     uint32_t again = (uint32_t)votes | (uint32_t)(votes >> 32);
@@ -329,7 +334,7 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
         float *po = p.part_o + w.slot * a.D;
         TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 if (32 * d + 8 * r4 >= a.D) continue;   // (D is a multiple of 8)
@@ -379,7 +384,7 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p,
         }
         // a row's threads are neighbours in one wave: any of their votes counts
         const float all = (x[0] + x[1]) + (x[2] + x[3]) + l;
-        uint64_t again = __ballot(ok && all != all);
+        uint64_t again = __ballot(ok && 4 * c < a.D && all != all);
         if (again) {
 #pragma unroll
             for (int sft = 1; sft < PIECES; sft <<= 1) again |= again >> sft;
@@ -471,12 +476,12 @@ __device__ __forceinline__ uint32_t piece_off(int place, int swz, int D) { retur
 // have no mask, and may have a cap)
 enum AttnKind { OWN, OWN_GENERAL, OWN_BEHIND, PREFIX_KEYS };
 
-template <typename TK, typename TQ, int DP, int WAVES, bool BY_ROWS, AttnKind KIND>
+template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS, AttnKind KIND>
 __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p, char *lds, int id) {
-    using T = AttnTile<TK, TQ, DP, WAVES, BY_ROWS>;
+    using T = AttnTile<TK, TQ, DC, WAVES, BY_ROWS>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
-    constexpr int KT = T::KT, CPR = T::CPR, RPD = T::RPD, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DP / 16, NB = DP / 32;
+    constexpr int DP = T::DP, KT = T::KT, CPR = T::CPR, RPD = T::RPD, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DC / 16, NB = DC / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     // problem, row tile (the last ones first: with a causal rule they see the most keys), split of the keys
     const int bh = p.by_bh.rest(id), at = p.by_bh.of(id), behind = p.by_split.of(at);
@@ -612,6 +617,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         }
     }
     c = fmaxf(c, 0x1p-126f);
+    // a mask alone joins the bare products, by the slope over their factor, where that is no extreme number
+    const bool scaled = capped || (masked && __any(!(c > 0x1p-60f && c < 0x1p20f)));
+    if (masked && !scaled) slope /= c;
     __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
 
     f32x16 o[NB];
@@ -702,7 +710,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     auto weights = [&](int j, const f16x4 (&w)[KT / 8]) {
         const int left = seen - j - 4 * h;
         float f = c;
-        if (capped || masked) {
+        if (scaled) {
             const float by = capped ? c_cap : c;
             f = 1.0f;
 #pragma unroll
@@ -754,6 +762,10 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             }
         l += sum;
     };
+    // (-1 that the compiler does not see: a second term is then one mixed fma, not a conversion, a difference and
+    // another conversion)
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
     auto values = [&](const char *vt) {
         // O^T += V^T P^T, 16 keys a step: the lane's weights 8 (t % 2) .. + 7 of block t / 2
         const int vi = lane & 15, vrow = 4 * h + (vi >> 2), vch = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1), vsw = swz_v<DP>(vrow);
@@ -761,10 +773,17 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         for (int t = 0; t < KT / 16; ++t) {
             x8 pf, pl;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = s[t / 2][8 * (t % 2) + e];
-                pf[e] = (TK)x;
-                if constexpr (SPLIT) pl[e] = (TK)(x - (float)pf[e]);
+            for (int e = 0; e < 8; e += 2) {
+                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                typedef TK x2 __attribute__((ext_vector_type(2)));
+                const f32x2 x = {s[t / 2][8 * (t % 2) + e], s[t / 2][8 * (t % 2) + e + 1]};
+                const x2 hi = __builtin_convertvector(x, x2);
+                pf[e] = hi[0];
+                pf[e + 1] = hi[1];
+                if constexpr (SPLIT) {
+                    pl[e] = (TK)fmaf(minus, (float)hi[0], x[0]);
+                    pl[e + 1] = (TK)fmaf(minus, (float)hi[1], x[1]);
+                }
             }
 #pragma unroll
             for (int d = 0; d < NB; ++d) {
@@ -874,7 +893,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         __syncthreads();
         join_waves<TK, TQ, DP, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
     } else {
-        store_rows<TK, TQ, DP, PREFIX>(a, p, o, me, l, row, row_ok, bh, split, j_begin, j_end);
+        store_rows<TK, TQ, DC, PREFIX>(a, p, o, me, l, row, row_ok, bh, split, j_begin, j_end);
     }
 }
 
@@ -882,20 +901,20 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 // by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs. 8 waves on a
 // CU: two workgroups of 4, which take turns at the matrix cores, or one of 8, which loads each tile of keys
 // for twice the rows; 4 where the largest heads' accumulators leave room for no more.
-template <typename TK, typename TQ, int DP, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL>
-__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
-    constexpr int L0 = AttnTile<TK, TQ, DP, WAVES, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DP, WAVES, PRE == 2>::LDS;
+template <typename TK, typename TQ, int DC, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL>
+__global__ __launch_bounds__(WAVES * 64, DC == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
+    constexpr int L0 = AttnTile<TK, TQ, DC, WAVES, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DC, WAVES, PRE == 2>::LDS;
     __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
     if constexpr (PRE != 0) {
         if ((int)blockIdx.x < pre.blocks) {
-            attn_tiles<TK, TQ, DP, WAVES, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
+            attn_tiles<TK, TQ, DC, WAVES, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
             return;
         }
     }
-    attn_tiles<TK, TQ, DP, WAVES, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
+    attn_tiles<TK, TQ, DC, WAVES, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
 }
 
-template <typename TK, typename TQ, int DP>
+template <typename TK, typename TQ, int DC>
 static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
     const int G = (int)a.by_G.d;
     AttnPart own{}, pre{};
@@ -920,9 +939,9 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     own.blocks = a.B * a.Hk * own.row_tiles * pl.own_splits;
     const bool general = a.mask != nullptr || a.cap != 0.0f;
     const dim3 grid((unsigned)(pre.blocks + own.blocks));
-    constexpr int WIDE = DP == 256 ? 4 : 8;
+    constexpr int DP = row_place(DC), WIDE = DP == 256 ? 4 : 8;
 #define ATTN_CASE(WAVES, PRE, ROWS, GENERAL) \
-    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DP, WAVES, PRE, ROWS, GENERAL>), grid, dim3(WAVES * 64), 0, st, a, pre, own)
+    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DC, WAVES, PRE, ROWS, GENERAL>), grid, dim3(WAVES * 64), 0, st, a, pre, own)
     if (pl.pre_splits) {
         if (!pl.pre_rows) ATTN_CASE(4, 1, false, false);
         else if (!pl.own_rows) ATTN_CASE(4, 2, false, false);
@@ -951,9 +970,9 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     }
 }
 
-template <typename TK, typename TQ, int DP>
+template <typename TK, typename TQ, int DC>
 static hipError_t launch_attn_any(const AttnArgs &a, const AttnPlan &pl, void *work, hipStream_t st) {
-    if (pl.tiled) launch_attn<TK, TQ, DP>(a, pl, work, st);
+    if (pl.tiled) launch_attn<TK, TQ, DC>(a, pl, work, st);
     else hipLaunchKernelGGL((attn_rows_kernel<TQ, TK>), dim3(a.n_q, a.H, a.B), dim3(256), 0, st, a);
     return hipGetLastError();
 }
