@@ -89,28 +89,35 @@ static AttnPlan plan_attn(const AttnTensors &t) {
         if (x && x->nb[1] >= (1u << 24)) p.tiled = false;
     if (!p.tiled) return p;
     // Splits of the keys, and workgroups of 4 or of 8 waves: the fewest us by a model of the launch.
-    //   a workgroup of row tiles: 7 us (8 waves: 9), and per tile of 64 keys 1.7 alone on its CU, 2.3 beside another
-    //     one (4 waves, 128 rows), 2.25 with 8 waves (256 rows); half for heads of up to 64 values, twice for f32
-    //     activations
+    //   a workgroup of row tiles with heads of 128 values: 4 waves, 128 rows 7 us, and per tile of 64 keys 1.4 alone
+    //     on its CU, 2.0 beside another one, 2.3 beside split keys; 8 waves, 256 rows 9 and 1.92; 8 waves, 128 rows,
+    //     two tiles at a time 8 and 1.85 for both, 2.05 where there are more workgroups than CUs. Of a tile's time
+    //     0.55 (8 waves: 0.65) up to 64 values, 0.83 up to 96; 1.8 for f32 activations. The rows of a causal call (the
+    //     rule is not known here: taken for one) see fewer keys, the last tiles the most
     //   a workgroup of split keys: 5 us, and per 128 keys what one CU draws from HBM, 1.6 (1.1 up to 64 values); all
     //     of them no less than their bytes at 5.5 TB/s, which fewer than 256 workgroups do not reach
     //   a prefix's workgroups are dealt first, then the batches' own, 512 (256 wide ones) at a time
-    //   more than one partial result a row: 4 for the second launch, and their trip through memory
+    //   more than one partial result a row: 5 for the second launch, and their trip through memory
     // Measured / by the model, us: one token, 8 key heads of 128 values, 8192 keys, 1 / 4 / 16 / 32 / 64 splits 85.7,
     // 30.9, 17.2, 16.9, 19.2 / 107, 35, 17, 18, 21; 131072 keys, 16 / 24 / 32 / 64 splits 122, 116, 105, 106 / 131, 119,
     // 110, 116; 64 sequences behind 8192 shared keys, 6 / 8 / 16 splits of them 54, 46, 53 / 65, 52, 58; 16 x 4 draft
-    // tokens behind 32768, 24 / 28 / 32 splits 62, 58, 68 / 72, 72, 79.
+    // tokens behind 32768, 24 / 28 / 32 splits 62, 58, 68 / 72, 72, 79. Row tiles, 4 waves / 8 / two tiles at a time: 32
+    // causal heads of 8192 tokens 547, 533, 588 / 526, 510, 557; of 2048 60, 61, 50 / 71, 70, 41; 16 of 512 behind 512
+    // 27.9, 33.2, 22.8 / 29, 40, 23, the latter's 2 and 4 splits 23.9, 24.9 / 24, 23.
     const int64_t D = t.q.ne[0], rows = n_q * G;
-    const double size = (D <= 64 ? 0.5 : D <= 96 ? 0.8 : 1.0) * (t.q.type == T_F32 ? 2.0 : 1.0);
-    struct Part { double groups, alone, beside, bytes; int tiles; };   // workgroups, us of each, bytes of split keys
-    auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int s) {
-        const int64_t per_tile = by_rows ? waves * 32 : 32, step = by_rows ? (D <= 128 ? 64 : 32) : 128;
+    const double size = t.q.type == T_F32 ? 1.8 : 1.0, size4 = size * (D <= 64 ? 0.55 : D <= 96 ? 0.83 : 1.0), size8 = size * (D <= 64 ? 0.65 : D <= 96 ? 0.83 : 1.0);
+    // workgroups, us of each alone on its CU and not, bytes of split keys
+    struct Part { double groups, alone, beside, bytes; int tiles; };
+    auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int turns, int s) {
+        const int64_t per_tile = by_rows ? waves / turns * 32 : 32, step = by_rows ? (D <= 128 ? 64 * turns : 32) : 128;
         const int tiles = (int)((rows + per_tile - 1) / per_tile);
         const double groups = (double)problems * tiles * s, n = std::ceil(std::ceil((double)keys / s) / step);
         if (!by_rows) return Part{groups, 5.0 + n * (D <= 64 ? 1.1 : 1.6), 0.0, (double)problems * keys * D * 4, tiles};
-        if (waves == 8) return Part{groups, 9.0 + n * 2.25 * size, 9.0 + n * 2.25 * size, 0.0, tiles};
-        return Part{groups, 7.0 + n * 1.7 * size, 7.0 + n * 2.3 * size, 0.0, tiles};
+        if (turns == 2) return Part{groups, 8.0 + n * 1.85 * size8, 8.0 + n * 2.05 * size8, 0.0, tiles};
+        if (waves == 8) return Part{groups, 9.0 + n * 1.92 * size8, 9.0 + n * 1.92 * size8, 0.0, tiles};
+        return Part{groups, 7.0 + n * 1.4 * size4, 7.0 + n * (t.kp ? 2.3 : 2.0) * size4, 0.0, tiles};
     };
+    const double fewer = t.k.ne[1] > 0 ? std::min(1.0, (double)n_q / (double)t.k.ne[1]) : 0.0;   // of the first rows, causal
     auto launch = [&](const Part &pre, const Part &own, int waves) {
         const double at_once = D > 128 || waves == 8 ? 256.0 : 512.0, all = pre.groups + own.groups;
         auto us = [&](const Part &x) { return x.bytes == 0.0 && all > 256.0 ? x.beside : x.alone; };
@@ -120,34 +127,43 @@ static AttnPlan plan_attn(const AttnTensors &t) {
         const double memory = bytes == 0.0 ? 0.0
                                            : 5.0 + bytes / rate + 3.0 * ((pre.bytes > 0.0 ? pre.groups : 0.0) + (own.bytes > 0.0 ? own.groups : 0.0)) / 512.0 +
                                                  (pre.groups > 0.0 && pre.bytes == 0.0 ? pre.groups * pre_us / at_once : 0.0);
-        if (pre.groups == 0.0) return std::max(memory, std::ceil(own.groups / at_once) * (own.bytes == 0.0 ? own_us : 0.0) + (own.bytes == 0.0 ? 0.0 : own_us));
+        if (pre.groups == 0.0) {
+            const double rounds = own.groups / at_once;
+            if (own.bytes != 0.0) return std::max(memory, own_us);
+            return std::max(own_us, own_us * ((1.0 - fewer / 2) * rounds + (1.0 - fewer) * (std::ceil(rounds) - rounds)));
+        }
         // the prefix's whole rounds, the rest of it with own ones beside it, then the others wherever one ends first
         const double before = std::floor(pre.groups / at_once) * pre_us, left = std::fmod(pre.groups, at_once), beside = at_once - left;
         const double end = before + (left > 0.0 ? pre_us : 0.0), rest = own.groups - beside;
         if (rest <= 0.0) return std::max({memory, end, before + own_us});
         return std::max({memory, end, std::min(before + own_us * (1.0 + std::ceil(rest / beside)), end + own_us * std::ceil(rest / at_once))});
     };
-    auto join = [&](int slots) { return slots > 1 ? 4.0 + (double)B * H * n_q * slots * D * 8 / 5e6 : 0.0; };
+    auto join = [&](int slots) { return slots > 1 ? 5.0 + (double)B * H * n_q * slots * D * 8 / 5e6 : 0.0; };
     static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 28, 32, 48, 64, 96, 128};
     static_assert(128 <= ATTN_MAX_SLOTS / 2, "a prefix's splits and the batches' own");
-    const int wide = D <= 128 ? 8 : 4;
     p.own_rows = rows > 32;
     p.pre_rows = t.kp && B * rows > 32;
     const int64_t n_kv = t.k.ne[1], n_pre = t.kp ? t.kp->ne[1] : 0;
     double best = 0.0;
     // (row tiles may gain by the wide workgroups; split keys do not, and beside them two smaller ones do better)
-    for (int waves = t.kp && p.own_rows ? wide : 4; waves <= (p.own_rows ? wide : 4); waves += 4)
+    struct Kind { int waves, turns; };
+    static const Kind KINDS[] = {{4, 1}, {8, 1}, {8, 2}};
+    for (const Kind &w : KINDS) {
+        const bool wide = w.waves == 8;
+        if (wide && (!p.own_rows || D > 128)) continue;
+        if (t.kp && (w.turns > 1 || (p.own_rows && D <= 128 && !wide))) continue;
         for (int so : SPLITS) {
             if (so > 1 && ((so - 1) * 32 >= n_kv || (t.kp && so > 4))) break;
-            const Part own = part(rows, B * Hk, n_kv, p.own_rows, waves, so);
+            const Part own = part(rows, B * Hk, n_kv, p.own_rows, w.waves, w.turns, so);
             for (int sp : SPLITS) {
                 if (sp > 1 && (sp - 1) * 32 >= n_pre) break;
-                const Part pre = t.kp ? part(B * rows, Hk, n_pre, p.pre_rows, waves, sp) : Part{};
+                const Part pre = t.kp ? part(B * rows, Hk, n_pre, p.pre_rows, w.waves, 1, sp) : Part{};
                 const int slots = t.kp ? so + sp : so;
-                const double us = launch(pre, own, waves) + join(slots);
+                const double us = launch(pre, own, w.waves) + join(slots);
                 if (p.slots != 0 && us >= best) continue;
                 best = us;
-                p.waves = waves;
+                p.waves = w.waves;
+                p.turns = w.turns;
                 p.own_splits = so;
                 p.own_tiles = own.tiles;
                 p.pre_splits = t.kp ? sp : 0;
@@ -155,6 +171,7 @@ static AttnPlan plan_attn(const AttnTensors &t) {
                 p.slots = slots;
             }
         }
+    }
     return p;
 }
 

@@ -42,7 +42,7 @@ constexpr int ATTN_MAX_SLOTS = 256;   // partial results of a row
 // what a call launches, by its shapes alone
 struct AttnPlan {
     bool tiled;                              // else attn_rows_kernel
-    int waves;                               // of a workgroup
+    int waves, turns;                        // of a workgroup; groups of its waves that have the same rows
     bool own_rows, pre_rows;                 // row tiles of 32 per wave, or 32 rows whose keys the waves split
     int own_tiles, own_splits, pre_tiles, pre_splits, slots;
 };

@@ -216,20 +216,20 @@ __device__ __forceinline__ void dma16(int u, i32x4 buf, const char *dst, uint32_
 // behind the row is a copy of its last piece, and no product reads it beyond DC)
 constexpr int row_place(int DC) { return DC <= 64 ? 64 : DC <= 128 ? 128 : 256; }
 
-template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS>
+template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS, int TURNS = 1>
 struct AttnTile {
     static constexpr bool SPLIT = sizeof(TQ) == 4;
     static constexpr int DP = row_place(DC);
     static constexpr int KT = BY_ROWS && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int CPR = DP / 8;                          // 16-byte pieces of a row
     static constexpr int RPD = 64 / CPR;                        // rows of a DMA
-    static constexpr int ROUNDS = KT / RPD / (BY_ROWS ? WAVES : 1);   // a wave's DMAs of a tile of keys, or of values
+    static constexpr int ROUNDS = KT / RPD / (BY_ROWS ? WAVES / TURNS : 1);   // a wave's DMAs of a tile of keys, or of values
     static constexpr int BYTES = KT * DP * 2;                   // of a tile of keys, and of values
     // BY_ROWS: two stages of keys and values; else one of each per wave, whose 32 rows also fit it as f32,
     // and those rows' maxima and sums
     static constexpr int STRETCH = BY_ROWS ? 4 * BYTES : 2 * BYTES + 256;
-    static constexpr int LDS = (BY_ROWS ? 1 : WAVES) * STRETCH;
-    static constexpr int STEP = BY_ROWS ? KT : WAVES * 32;      // keys that a workgroup takes at a time
+    static constexpr int LDS = (BY_ROWS ? TURNS : WAVES) * STRETCH;
+    static constexpr int STEP = BY_ROWS ? TURNS * KT : WAVES * 32;   // keys that a workgroup takes at a time
     typedef typename Vec<TK>::x8 x8;
 };
 
@@ -476,9 +476,9 @@ __device__ __forceinline__ uint32_t piece_off(int place, int swz, int D) { retur
 // have no mask, and may have a cap)
 enum AttnKind { OWN, OWN_GENERAL, OWN_BEHIND, PREFIX_KEYS };
 
-template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS, AttnKind KIND>
+template <typename TK, typename TQ, int DC, int WAVES, bool BY_ROWS, AttnKind KIND, int TURNS>
 __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p, char *lds, int id) {
-    using T = AttnTile<TK, TQ, DC, WAVES, BY_ROWS>;
+    using T = AttnTile<TK, TQ, DC, WAVES, BY_ROWS, TURNS>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
     constexpr int DP = T::DP, KT = T::KT, CPR = T::CPR, RPD = T::RPD, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DC / 16, NB = DC / 32;
@@ -488,8 +488,10 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int split = at - behind * (int)p.by_split.d, tile = p.row_tiles - 1 - behind;
     const int G = (int)a.by_G.d, pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk;
 
-    // this lane's row
-    const int row0 = (BY_ROWS ? tile * WAVES + wave : tile) * 32;
+    // this lane's row (TURNS groups of RW waves have the same rows, and take turns at the tiles of keys)
+    constexpr int RW = WAVES / TURNS;
+    const int turn = BY_ROWS ? wave / RW : 0, rwave = BY_ROWS ? wave % RW : wave;
+    const int row0 = (BY_ROWS ? tile * RW + rwave : tile) * 32;
     const int row = min(row0 + (lane & 31), p.rows - 1);
     const bool row_ok = row0 + (lane & 31) < p.rows;
     const int bi = a.by_G.of(row), head = hk * G + row - bi * G;
@@ -523,7 +525,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const int n = PREFIX ? a.n_prefix : own_len(a, b);
     int end = n;                                    // of the workgroup's rows
     if (!PREFIX && a.causal) {
-        const int last = min((BY_ROWS ? (tile + 1) * WAVES : tile + 1) * 32 - 1, p.rows - 1);
+        const int last = min((BY_ROWS ? (tile + 1) * RW : tile + 1) * 32 - 1, p.rows - 1);
         end = max(0, n - a.n_q + a.by_G.of(last) + 1);
     }
     int j_begin = 0, j_end = end;
@@ -552,8 +554,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 
     // the tile at key j into `dst`, this wave's (BY_ROWS: the workgroup's) LDS
     // (its waves take ROUNDS pieces of RPD rows each)
-    const int lrow = lane / CPR, place = lane % CPR, first = BY_ROWS ? wave * ROUNDS : 0;
-    char *stage0 = lds + (BY_ROWS ? 0 : wave * T::STRETCH);
+    const int lrow = lane / CPR, place = lane % CPR, first = BY_ROWS ? rwave * ROUNDS : 0;
+    char *stage0 = lds + (BY_ROWS ? turn : wave) * T::STRETCH;
     const uint32_t k_row = lrow * (uint32_t)k_j, v_row = lrow * (uint32_t)v_j;
     auto load = [&](const char *base, int64_t stride, uint32_t row0, int j, char *dst, auto swz) {
         const char *to = dst + first * 1024;
@@ -575,7 +577,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     auto load_k = [&](int j, char *dst) { load(kb, k_j, k_row, j, dst, [](int r) { return swz_k<DP>(r); }); };
     auto load_v = [&](int j, char *dst) { load(vb, v_j, v_row, j, dst, [](int r) { return swz_v<DP>(r); }); };
 
-    const int j0 = BY_ROWS ? j_begin : j_begin + wave * 32;
+    const int j0 = j_begin + (BY_ROWS ? turn * KT : wave * 32);
     if (j0 < j_end) {
         load_k(j0, stage0);
         load_v(j0, stage0 + BYTES);
@@ -679,7 +681,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         __builtin_amdgcn_sched_group_barrier(0x008, PER * AHEAD, 0);
     };
     // the same with the next tile's DMA (a whole one, into `to`) dealt out among the MFMAs: issued in a row it holds a
-    // wave up for 1000 cycles, a quarter of a tile's time
+    // wave up for hundreds of cycles, a tenth of a tile's time
     auto products_and_load = [&](const char *kt, int j, char *to) {
         constexpr int NQK = KT / 32 * NT, EVERY = NQK / (2 * ROUNDS) > 0 ? NQK / (2 * ROUNDS) : 1;
         static_assert(!BY_ROWS || 2 * ROUNDS * EVERY <= NQK, "every DMA has its step");
@@ -809,9 +811,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         // (a later row sees no fewer keys)
         const int seen_most = row0 < p.rows ? __builtin_amdgcn_readlane(seen, 31) : 0;
         f16x4 w[KT / 8], ahead[KT / 8];
-        if (masked && j_begin < j_end) fetch(j_begin, ahead);
+        if (masked && j0 < j_end) fetch(j0, ahead);
         char *now = stage0, *next = stage0 + 2 * BYTES;
-        for (int j = j_begin; j < j_end; j += KT) {
+        for (int j = j0; j - turn * KT < j_end; j += T::STEP) {   // (as often for every wave)
             // this wave's share of the tile has come; behind the barrier everyone's has, and the other stage is read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (masked) {   // (moved here, so that the compiler's wait for them comes before the next DMA)
@@ -821,17 +823,17 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                     asm volatile("" : "+v"(w[r]));
                 }
             }
-            // (8 waves have half the DMA each, and lose 3 % by dealing it out)
-            const bool mine = j < seen_most && !(masked && hidden(w)), among = WAVES == 4 && mine && j + 2 * KT <= j_end;
-            if (j + KT < j_end && !among) {
-                load_k(j + KT, next);
-                load_v(j + KT, next + BYTES);
+            // (8 waves that share a tile have half the DMA each, and lose 3 % by dealing it out)
+            const bool mine = j < seen_most && !(masked && hidden(w)), among = RW == 4 && mine && j + T::STEP + KT <= j_end;
+            if (j + T::STEP < j_end && !among) {
+                load_k(j + T::STEP, next);
+                load_v(j + T::STEP, next + BYTES);
             }
-            if (masked && j + KT < j_end) fetch(j + KT, ahead);
+            if (masked && j + T::STEP < j_end) fetch(j + T::STEP, ahead);
             if (mine) {
                 // (a wave that feeds the matrix cores goes before one that forms weights)
                 __builtin_amdgcn_s_setprio(1);
-                if (among) products_and_load(now, j + KT, next);
+                if (among) products_and_load(now, j + T::STEP, next);
                 else products(now);
                 __builtin_amdgcn_s_setprio(0);
                 weights(j, w);
@@ -872,7 +874,6 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         }
     }
     l += swap32_f(l);
-    const float me = m - BIAS;   // (-inf: no key)
 
     if constexpr (!BY_ROWS) {
         // join the waves: each leaves its rows in its own stretch
@@ -886,32 +887,66 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                     *reinterpret_cast<f32x4 *>(stage0 + piece_at<DP>(lane & 31, 8 * d + 2 * r4 + h)) =
                         f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
             if (h == 0) {
-                pm[lane] = me;
+                pm[lane] = m - BIAS;   // (-inf: no key)
                 pm[32 + lane] = l;
             }
         }
         __syncthreads();
         join_waves<TK, TQ, DP, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
     } else {
-        store_rows<TK, TQ, DC, PREFIX>(a, p, o, me, l, row, row_ok, bh, split, j_begin, j_end);
+        if constexpr (TURNS > 1) {
+            // the second group leaves its part to the first one, in LDS that no DMA is on its way to: the rows' maxima
+            // and sums, and its accumulators in order of the lanes
+            static_assert(TURNS == 2 && RW * (NB * 4096 + 512) <= T::LDS, "a wave's accumulators, maxima and sums");
+            char *mine = lds + rwave * (NB * 4096 + 512);
+            __syncthreads();
+            if (turn == 1) {
+                float *ml = reinterpret_cast<float *>(mine + NB * 4096);
+                ml[lane] = m;
+                ml[64 + lane] = l;
+#pragma unroll
+                for (int d = 0; d < NB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        reinterpret_cast<f32x4 *>(mine)[(4 * d + r) * 64 + lane] = f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+            }
+            __syncthreads();
+            if (turn == 1) return;
+            const float *ml = reinterpret_cast<const float *>(mine + NB * 4096);
+            const float m1 = ml[lane], top = fmaxf(m, m1);
+            const float f0 = m == top ? 1.0f : exp2f(m - top), f1 = m1 == top ? 1.0f : exp2f(m1 - top);
+            l = l * f0 + ml[64 + lane] * f1;
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 x = reinterpret_cast<const f32x4 *>(mine)[(4 * d + r) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][4 * r + e] = o[d][4 * r + e] * f0 + x[e] * f1;
+                }
+            m = top;
+        }
+        store_rows<TK, TQ, DC, PREFIX>(a, p, o, m - BIAS, l, row, row_ok, bh, split, j_begin, j_end);
     }
 }
 
 // One launch: the workgroups of a shared prefix (PRE: 0 none, 1 split keys, 2 row tiles), which are bound
 // by the matrix cores, then those of the batches' own keys, bound by memory, on the same CUs. 8 waves on a
 // CU: two workgroups of 4, which take turns at the matrix cores, or one of 8, which loads each tile of keys
-// for twice the rows; 4 where the largest heads' accumulators leave room for no more.
-template <typename TK, typename TQ, int DC, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL>
+// for twice the rows, or (TURNS = 2) whose halves have the same rows, work on two tiles of keys and join what they have
+// in LDS: half the splits, or none, where row tiles are few. 4 where the largest heads' accumulators leave room for
+// no more. Causal heads of 128 values, 32 on 8, 2048 tokens: 60 us by 4 waves, 61 by 8, 50 in turns; 8192: 547, 533, 588.
+template <typename TK, typename TQ, int DC, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL, int TURNS>
 __global__ __launch_bounds__(WAVES * 64, DC == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
-    constexpr int L0 = AttnTile<TK, TQ, DC, WAVES, OWN_ROWS>::LDS, L1 = AttnTile<TK, TQ, DC, WAVES, PRE == 2>::LDS;
+    constexpr int L0 = AttnTile<TK, TQ, DC, WAVES, OWN_ROWS, TURNS>::LDS, L1 = AttnTile<TK, TQ, DC, WAVES, PRE == 2>::LDS;
     __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
     if constexpr (PRE != 0) {
         if ((int)blockIdx.x < pre.blocks) {
-            attn_tiles<TK, TQ, DC, WAVES, PRE == 2, PREFIX_KEYS>(a, pre, lds, blockIdx.x);
+            attn_tiles<TK, TQ, DC, WAVES, PRE == 2, PREFIX_KEYS, 1>(a, pre, lds, blockIdx.x);
             return;
         }
     }
-    attn_tiles<TK, TQ, DC, WAVES, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
+    attn_tiles<TK, TQ, DC, WAVES, OWN_ROWS, PRE ? OWN_BEHIND : GENERAL ? OWN_GENERAL : OWN, TURNS>(a, own, lds, blockIdx.x - (PRE ? pre.blocks : 0));
 }
 
 template <typename TK, typename TQ, int DC>
@@ -940,20 +975,23 @@ static void launch_attn(const AttnArgs &a, const AttnPlan &pl, void *work, hipSt
     const bool general = a.mask != nullptr || a.cap != 0.0f;
     const dim3 grid((unsigned)(pre.blocks + own.blocks));
     constexpr int DP = row_place(DC), WIDE = DP == 256 ? 4 : 8;
-#define ATTN_CASE(WAVES, PRE, ROWS, GENERAL) \
-    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DC, WAVES, PRE, ROWS, GENERAL>), grid, dim3(WAVES * 64), 0, st, a, pre, own)
+#define ATTN_CASE(WAVES, PRE, ROWS, GENERAL, TURNS) \
+    hipLaunchKernelGGL((attn_tile_kernel<TK, TQ, DC, WAVES, PRE, ROWS, GENERAL, TURNS>), grid, dim3(WAVES * 64), 0, st, a, pre, own)
     if (pl.pre_splits) {
-        if (!pl.pre_rows) ATTN_CASE(4, 1, false, false);
-        else if (!pl.own_rows) ATTN_CASE(4, 2, false, false);
-        else ATTN_CASE(WIDE, 2, true, false);
+        if (!pl.pre_rows) ATTN_CASE(4, 1, false, false, 1);
+        else if (!pl.own_rows) ATTN_CASE(4, 2, false, false, 1);
+        else ATTN_CASE(WIDE, 2, true, false, 1);
     } else if (pl.waves == 4) {
-        if (pl.own_rows && general) ATTN_CASE(4, 0, true, true);
-        else if (pl.own_rows) ATTN_CASE(4, 0, true, false);
-        else if (general) ATTN_CASE(4, 0, false, true);
-        else ATTN_CASE(4, 0, false, false);
+        if (pl.own_rows && general) ATTN_CASE(4, 0, true, true, 1);
+        else if (pl.own_rows) ATTN_CASE(4, 0, true, false, 1);
+        else if (general) ATTN_CASE(4, 0, false, true, 1);
+        else ATTN_CASE(4, 0, false, false, 1);
+    } else if (pl.turns == 2) {
+        if (general) ATTN_CASE(WIDE, 0, true, true, WIDE / 4);
+        else ATTN_CASE(WIDE, 0, true, false, WIDE / 4);
     } else {
-        if (general) ATTN_CASE(WIDE, 0, true, true);
-        else ATTN_CASE(WIDE, 0, true, false);
+        if (general) ATTN_CASE(WIDE, 0, true, true, 1);
+        else ATTN_CASE(WIDE, 0, true, false, 1);
     }
 #undef ATTN_CASE
     if (pl.slots > 1) {

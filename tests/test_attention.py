@@ -260,6 +260,48 @@ def test_nan_and_infinity_that_a_row_sees(kv, io):
     assert ((rows.double() - o[0][keep.cuda()]).abs() <= most[0][keep.cuda()])[:, others].all()
 
 
+LAUNCHES = [
+    # B, n_q, n_kv, H, Hk, D: few row tiles, one for each CU, several (workgroups of 4 and 8 waves, their tiles of keys
+    # shared or taken in turns, the keys split or not)
+    (1, 300, 3000, 8, 2, 64), (1, 515, 1031, 16, 4, 128), (1, 300, 1500, 32, 8, 96), (1, 1024, 1030, 32, 8, 128), (1, 2049, 2049, 16, 8, 88),
+    (2, 2048, 2050, 32, 4, 64), (2, 2048, 2048, 32, 4, 128), (4, 700, 900, 32, 8, 96), (2, 777, 1900, 16, 16, 80), (1, 600, 1000, 16, 2, 256),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("size", LAUNCHES, ids=lambda s: "x".join(map(str, s)))
+def test_row_tiles_of_every_launch(size, kv, io):
+    """plain, causal with ragged lengths (one of none) and sinks, and masked with a cap, hidden NaN and rows that see
+    nothing"""
+    B, n, m, H, Hk, D = size
+    q, k, v = operands(B, n, m, H, Hk, D, kv, io, seed=sum(size))
+    s = 1 / math.sqrt(D)
+    near(call(q, k, v, s), formula(q, k, v, s, full(B, m)))
+    lens = torch.tensor([0 if i == 3 else max(0, m - 333 * i) for i in range(B)], dtype=torch.int32, device="cuda")
+    sinks = rnd((H,), "f32", 5)
+    near(call(q, k, v, s, lens=lens, causal=True, sinks=sinks), formula(q, k, v, s, lens, causal=True, sinks=sinks))
+    w = rnd((1, 1, n, m), "f16", 8)
+    w[0, 0, :, 5::3] = -INF
+    w[0, 0, n // 2, :] = -INF
+    w[0, 0, : min(n, 200), 128 : 128 + m // 2] = -INF
+    k[:, 5::3], v[:, 5::3] = NAN, NAN
+    near(call(q, k, v, s, mask=w, cap=20.0), formula(q, k, v, s, full(B, m), mask=w, cap=20.0))
+    near(call(q, k, v, s, mask=w, bias=4.0), formula(q, k, v, s, full(B, m), mask=w, bias=4.0))
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("scale", [0.0, 1e-25, -0.125, 3.0e6])
+def test_masks_beside_extreme_scales(kv, io, scale):
+    """products that next to nothing or far too much multiplies, next to a finite mask"""
+    q, k, v = operands(1, 70, 90, 2, 1, 64, kv, io, seed=31)
+    w = (rnd((1, 1, 70, 90), "f32", 32) * 50).to(torch.float16)
+    w[..., ::4] = -1000
+    w[..., 1::9] = -INF
+    near(call(q, k, v, scale, mask=w), formula(q, k, v, scale, full(1, 90), mask=w))
+
+
 @gpu
 @pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
 @pytest.mark.parametrize("n", [1, 50])
