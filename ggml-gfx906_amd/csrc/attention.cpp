@@ -219,7 +219,6 @@ int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t 
         a.mask = static_cast<const char *>(t.mask->data);
         a.m_i = (int64_t)t.mask->nb[1]; a.m_h = (int64_t)t.mask->nb[2]; a.m_b = (int64_t)t.mask->nb[3];
         a.m_nh = (int)t.mask->ne[2]; a.m_nb = (int)t.mask->ne[3];
-        a.m_vec = aligned_to(*t.mask, 8);
     }
     if (t.sinks) a.sinks = static_cast<const float *>(t.sinks->data);
     if (t.len) {

@@ -25,7 +25,6 @@ struct AttnArgs {
     const char *vp; int64_t vp_j, vp_h;
     const char *mask; int64_t m_i, m_h, m_b;         // f16, or nullptr
     int m_nh, m_nb;                                  // its head and batch planes
-    bool m_vec;                                      // rows of 8-byte aligned groups of four
     const float *sinks;
     const char *len; int64_t len_b;                  // i32 [batch], or nullptr: n_kv
     char *o; int64_t o_i, o_h, o_b;

@@ -631,10 +631,12 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 
     // the mask's values at the tile's keys, in the order of the scores
     auto fetch = [&](int j, f16x4 (&w)[KT / 8]) {
+        // (rows of a mask begin at any multiple of 2 bytes; the card's loads may)
+        typedef f16x4 f16x4_any __attribute__((aligned(2)));
         const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 4 * h;
-        if (a.m_vec && __all(seen - j >= KT)) {
+        if (__all(seen - j >= KT)) {
 #pragma unroll
-            for (int r = 0; r < KT / 8; ++r) w[r] = *reinterpret_cast<const f16x4 *>(mp + 8 * r);
+            for (int r = 0; r < KT / 8; ++r) w[r] = *reinterpret_cast<const f16x4_any *>(mp + 8 * r);
         } else {
             const int left = seen - j - 4 * h;
 #pragma unroll

@@ -70,56 +70,63 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     }
 }
 
-// Rows of whole groups of 8 values at 16-byte (f32) / 8-byte places: a thread turns the same 4 pairs of
-// HEADS heads of one token, so their sines are formed once, and all its loads are issued before them.
+// Rows of whole groups of 2 W values at the places of W: a thread turns the same W pairs of HEADS heads of one
+// token, so their sines are formed once, and all its loads are issued before them.
 // Bound by memory: 4096 tokens x 32 heads x 128 f32 values, 134 MB in 24.4 us, 5.5 TB/s; 8192 x 8 x 128 f32
 // into f16 12.4 us, 4.1 TB/s; a token's 32 heads 3.5 us, the launch.
-template <typename T> struct RopeVec { typedef T x4 __attribute__((ext_vector_type(4))); };
+template <typename T, int W> struct RopeVec { typedef T v __attribute__((ext_vector_type(W))); };
 
-template <typename TS, typename TD, bool HALVES, int HEADS>
+template <typename TS, typename TD, bool HALVES, int HEADS, int W>
 __global__ __launch_bounds__(256) void rope_vec_kernel(const RopeArgs a) {
-    typedef typename RopeVec<TS>::x4 S4;
-    typedef typename RopeVec<TD>::x4 D4;
-    const uint32_t units = (uint32_t)a.ne0 / 8, at = blockIdx.x * 256 + threadIdx.x;
+    typedef typename RopeVec<TS, W>::v SV;
+    typedef typename RopeVec<TD, W>::v DV;
+    const uint32_t units = (uint32_t)a.ne0 / (2 * W), at = blockIdx.x * 256 + threadIdx.x;
     const uint32_t t = at / units, u = at % units;
     if (t >= (uint32_t)a.ne2) return;
     const int h0 = blockIdx.y * HEADS, b = blockIdx.z;
-    const bool turns = u < (uint32_t)a.n_dims / 8;
-    // the two groups of four values
-    const int i0 = HALVES && turns ? 4 * u : 8 * u, i1 = HALVES && turns ? 4 * u + a.n_dims / 2 : 8 * u + 4;
+    const bool turns = u < (uint32_t)a.n_dims / (2 * W);
+    // the two groups of W values
+    const int i0 = HALVES && turns ? W * u : 2 * W * u, i1 = HALVES && turns ? W * u + a.n_dims / 2 : 2 * W * u + W;
     const char *s = a.src + (int64_t)t * a.s_t + b * a.s_b;
     char *d = a.dst + (int64_t)t * a.d_t + b * a.d_b;
-    S4 x[HEADS], y[HEADS];
+    SV x[HEADS], y[HEADS];
 #pragma unroll
     for (int k = 0; k < HEADS; ++k) {
         const TS *r = reinterpret_cast<const TS *>(s + min(h0 + k, a.ne1 - 1) * a.s_h);
-        x[k] = *reinterpret_cast<const S4 *>(r + i0);
-        y[k] = *reinterpret_cast<const S4 *>(r + i1);
+        x[k] = *reinterpret_cast<const SV *>(r + i0);
+        y[k] = *reinterpret_cast<const SV *>(r + i1);
     }
-    float cs[4] = {}, sn[4] = {};
+    float cs[W] = {}, sn[W] = {};
     if (turns) {
         const double pos = (double)a.pos[b * a.pos_b + t];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) turn(a, 4 * u + e, pos, cs[e], sn[e]);
+        for (int e = 0; e < W; ++e) turn(a, W * u + e, pos, cs[e], sn[e]);
     }
 #pragma unroll
     for (int k = 0; k < HEADS; ++k) {
         if (h0 + k >= a.ne1) break;
         TD *r = reinterpret_cast<TD *>(d + (h0 + k) * a.d_h);
-        float v[8], w[8];
+        float v[2 * W];
+        TD w[2 * W];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < W; ++e) {
             v[e] = (float)x[k][e];
-            v[4 + e] = (float)y[k][e];
+            v[W + e] = (float)y[k][e];
+        }
+        DV lo, hi;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+            const int ia = HALVES ? e : 2 * e, ib = HALVES ? e + W : 2 * e + 1;
+            w[ia] = (TD)(turns ? v[ia] * cs[e] - v[ib] * sn[e] : v[ia]);
+            w[ib] = (TD)(turns ? v[ia] * sn[e] + v[ib] * cs[e] : v[ib]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int ia = HALVES ? e : 2 * e, ib = HALVES ? e + 4 : 2 * e + 1;
-            w[ia] = turns ? v[ia] * cs[e] - v[ib] * sn[e] : v[ia];
-            w[ib] = turns ? v[ia] * sn[e] + v[ib] * cs[e] : v[ib];
+        for (int e = 0; e < W; ++e) {
+            lo[e] = w[e];
+            hi[e] = w[W + e];
         }
-        *reinterpret_cast<D4 *>(r + i0) = D4{(TD)w[0], (TD)w[1], (TD)w[2], (TD)w[3]};
-        *reinterpret_cast<D4 *>(r + i1) = D4{(TD)w[4], (TD)w[5], (TD)w[6], (TD)w[7]};
+        *reinterpret_cast<DV *>(r + i0) = lo;
+        *reinterpret_cast<DV *>(r + i1) = hi;
     }
 }
 
@@ -160,29 +167,35 @@ int rope_bytes(int t) { return t == T_F32 ? 4 : 2; }
 template <typename TS, typename TD>
 void rope_launch(const RopeArgs &g, int64_t batches, hipStream_t st) {
     auto fits = [](const void *p, int64_t h, int64_t t, int64_t b, int to) { return (uintptr_t)p % to == 0 && h % to == 0 && t % to == 0 && b % to == 0; };
-    const int64_t units = g.ne0 / 8, threads = units * g.ne2;
-    const bool vec = g.ne0 % 8 == 0 && g.n_dims % 8 == 0 && fits(g.src, g.s_h, g.s_t, g.s_b, 4 * sizeof(TS)) &&
-                     fits(g.dst, g.d_h, g.d_t, g.d_b, 4 * sizeof(TD)) && threads < (1LL << 31) && batches <= 65535 && g.ne1 <= 65535;
-    if (!vec) {
+    auto groups = [&](int w) {
+        return g.ne0 % (2 * w) == 0 && g.n_dims % (2 * w) == 0 && fits(g.src, g.s_h, g.s_t, g.s_b, w * (int)sizeof(TS)) &&
+               fits(g.dst, g.d_h, g.d_t, g.d_b, w * (int)sizeof(TD)) && (int64_t)(g.ne0 / (2 * w)) * g.ne2 < (1LL << 31) && batches <= 65535 &&
+               g.ne1 <= 65535;
+    };
+    const int w = groups(4) ? 4 : groups(2) ? 2 : groups(1) ? 1 : 0;
+    const int64_t threads = w ? (int64_t)(g.ne0 / (2 * w)) * g.ne2 : 0;
+    // One head a thread until that makes 4 waves for each SIMD of the 256 CUs; from there on the sines cost
+    // more than further waves hide, and a thread takes 8 heads (4 where there are fewer): 4096 x 32 x 128 f32
+    // 42.9 us with a pair a thread, 30.9 / 25.4 / 24.4 / 23.4 with 2 / 4 / 8 / 16 heads; 4 x 1000 x 20 x 80
+    // bf16 12.9 with one, 9.8 / 8.6 / 8.0 / 9.9. Rows that only fall into groups of 4 or of 2 values, 4 heads a thread:
+    // 3 x 3707 x 40 x 204 f16, 52 of them turned, 120 us (a pair a thread 354), 2000 x 32 x 102 f32 10.8 (18.0).
+    const int heads = threads * g.ne1 * batches < 4LL * 4 * 256 * 64 || g.ne1 == 1 ? 1 : g.ne1 < 8 || w < 4 ? 4 : 8;
+    if (w == 0 || (w < 4 && heads == 1)) {
         const int64_t n = g.rows * (g.n_dims / 2 + g.ne0 - g.n_dims);
         hipLaunchKernelGGL((rope_kernel<TS, TD>), dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, st, g);
         return;
     }
-    const unsigned blocks = (unsigned)((threads + 255) / 256);
-    // One head a thread until that makes 4 waves for each SIMD of the 256 CUs; from there on the sines cost
-    // more than further waves hide, and a thread takes 8 heads (4 where there are fewer): 4096 x 32 x 128 f32
-    // 42.9 us with a pair a thread, 30.9 / 25.4 / 24.4 / 23.4 with 2 / 4 / 8 / 16 heads; 4 x 1000 x 20 x 80
-    // bf16 12.9 with one, 9.8 / 8.6 / 8.0 / 9.9.
-    const int heads = threads * g.ne1 * batches < 4LL * 4 * 256 * 64 || g.ne1 == 1 ? 1 : g.ne1 < 8 ? 4 : 8;
-    const dim3 grid(blocks, (unsigned)((g.ne1 + heads - 1) / heads), (unsigned)batches);
-#define ROPE_CASE(N)                                                                                             \
-    if (heads == N) {                                                                                            \
-        if (g.halves) hipLaunchKernelGGL((rope_vec_kernel<TS, TD, true, N>), grid, dim3(256), 0, st, g);          \
-        else hipLaunchKernelGGL((rope_vec_kernel<TS, TD, false, N>), grid, dim3(256), 0, st, g);                  \
+    const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((g.ne1 + heads - 1) / heads), (unsigned)batches);
+#define ROPE_CASE(N, W)                                                                                              \
+    if (heads == N && w == W) {                                                                                      \
+        if (g.halves) hipLaunchKernelGGL((rope_vec_kernel<TS, TD, true, N, W>), grid, dim3(256), 0, st, g);           \
+        else hipLaunchKernelGGL((rope_vec_kernel<TS, TD, false, N, W>), grid, dim3(256), 0, st, g);                   \
     }
-    ROPE_CASE(1)
-    ROPE_CASE(4)
-    ROPE_CASE(8)
+    ROPE_CASE(1, 4)
+    ROPE_CASE(4, 4)
+    ROPE_CASE(8, 4)
+    ROPE_CASE(4, 2)
+    ROPE_CASE(4, 1)
 #undef ROPE_CASE
 }
 

@@ -84,6 +84,7 @@ SHAPES = [
     (1, 1, 1, 2, 2), (1, 1, 32, 128, 128), (1, 7, 3, 64, 64), (2, 33, 5, 80, 32), (1, 5, 2, 81, 18), (3, 129, 1, 96, 96),
     (1, 1000, 8, 128, 128), (2, 3, 4, 576, 512), (1, 17, 71, 20, 20), (1, 2, 1, 1000, 64), (1, 64, 1, 36, 34),
     (1, 2100, 13, 96, 96), (3, 4000, 3, 80, 40), (1, 1500, 20, 136, 64),   # several heads a thread, and their ends
+    (2, 3001, 9, 44, 36), (1, 4100, 6, 30, 14), (3, 1500, 7, 81, 40), (1, 2500, 5, 204, 52),   # groups of 4, of 2, of no values
 ]
 
 
