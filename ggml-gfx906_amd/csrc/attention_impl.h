@@ -629,21 +629,35 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     for (int d = 0; d < NB; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.0f;   // (l: of the lane's own keys)
 
-    // the mask's values at the tile's keys, in the order of the scores
-    auto fetch = [&](int j, f16x4 (&w)[KT / 8]) {
-        // (rows of a mask begin at any multiple of 2 bytes; the card's loads may)
-        typedef f16x4 f16x4_any __attribute__((aligned(2)));
-        const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 4 * h;
+    // the mask's values at the tile's keys, 8 in a row from one load: half the cache lines that 4 at a time ask for
+    // (rows of a mask begin at any multiple of 2 bytes; the card's loads may)
+    auto fetch = [&](int j, f16x8 (&w)[KT / 16]) {
+        typedef f16x8 f16x8_any __attribute__((aligned(2)));
+        const _Float16 *mp = reinterpret_cast<const _Float16 *>(mrow) + j + 8 * h;
         if (__all(seen - j >= KT)) {
 #pragma unroll
-            for (int r = 0; r < KT / 8; ++r) w[r] = *reinterpret_cast<const f16x4_any *>(mp + 8 * r);
+            for (int r = 0; r < KT / 16; ++r) w[r] = *reinterpret_cast<const f16x8_any *>(mp + 16 * r);
         } else {
-            const int left = seen - j - 4 * h;
+            const int left = seen - j - 8 * h;
 #pragma unroll
-            for (int r = 0; r < KT / 8; ++r)
+            for (int r = 0; r < KT / 16; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[r][e] = 8 * r + e < left ? mp[8 * r + e] : (_Float16)-INFINITY;
+                for (int e = 0; e < 8; ++e) w[r][e] = 16 * r + e < left ? mp[16 * r + e] : (_Float16)-INFINITY;
         }
+    };
+    // and in the order of the scores: the row's two lanes trade halves
+    auto arrange = [&](const f16x8 (&from)[KT / 16], f16x4 (&w)[KT / 8]) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int r = 0; r < KT / 16; ++r) {
+            const u32x4 x = __builtin_bit_cast(u32x4, from[r]);
+            const auto a0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), a1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+            w[2 * r] = __builtin_bit_cast(f16x4, u32x2{a0[0], a1[0]});
+            w[2 * r + 1] = __builtin_bit_cast(f16x4, u32x2{a0[1], a1[1]});
+        }
+#pragma unroll
+        for (int r = 0; r < KT / 8; ++r) asm volatile("" : "+v"(w[r]));   // here, behind the loads' wait and before the next DMA
     };
 
     // whether the mask hides the tile from all of the wave's rows
@@ -812,19 +826,14 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     if constexpr (BY_ROWS) {
         // (a later row sees no fewer keys)
         const int seen_most = row0 < p.rows ? __builtin_amdgcn_readlane(seen, 31) : 0;
-        f16x4 w[KT / 8], ahead[KT / 8];
+        f16x4 w[KT / 8];
+        f16x8 ahead[KT / 16];
         if (masked && j0 < j_end) fetch(j0, ahead);
         char *now = stage0, *next = stage0 + 2 * BYTES;
         for (int j = j0; j - turn * KT < j_end; j += T::STEP) {   // (as often for every wave)
             // this wave's share of the tile has come; behind the barrier everyone's has, and the other stage is read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (masked) {   // (moved here, so that the compiler's wait for them comes before the next DMA)
-#pragma unroll
-                for (int r = 0; r < KT / 8; ++r) {
-                    w[r] = ahead[r];
-                    asm volatile("" : "+v"(w[r]));
-                }
-            }
+            if (masked) arrange(ahead, w);
             // (8 waves that share a tile have half the DMA each, and lose 3 % by dealing it out)
             const bool mine = j < seen_most && !(masked && hidden(w)), among = RW == 4 && mine && j + T::STEP + KT <= j_end;
             if (j + T::STEP < j_end && !among) {
@@ -851,16 +860,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         // a tile's keys are refilled once their products are formed, its values behind those, so that either
         // is on its way while the other is worked on
         constexpr int STEP = T::STEP;
-        f16x4 w[KT / 8], ahead[KT / 8];
+        f16x4 w[KT / 8];
+        f16x8 ahead[KT / 16];
         if (masked && j0 < j_end) fetch(j0, ahead);
         for (int j = j0; j < j_end; j += STEP) {
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ROUNDS) : "memory");   // the keys
             if (masked) {
-#pragma unroll
-                for (int r = 0; r < KT / 8; ++r) {
-                    w[r] = ahead[r];
-                    asm volatile("" : "+v"(w[r]));
-                }
+                arrange(ahead, w);
                 if (j + STEP < j_end) fetch(j + STEP, ahead);
             }
             const bool idle = masked && hidden(w);
