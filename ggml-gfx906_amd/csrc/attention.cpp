@@ -48,8 +48,8 @@ static int check_attn(const AttnTensors &t, const AttnSpec &p) {
     for (int i = 1; i < 4; ++i)
         if (k.ne[i] != v.ne[i]) return GGML_MI355X_EINVAL;
     if (k.ne[2] <= 0 || H % k.ne[2] != 0 || k.ne[3] <= 0 || B % k.ne[3] != 0) return GGML_MI355X_EINVAL;
-    // (32-bit row and workgroup counts, with room for 512 splits or row tiles)
-    if (H > 65535 || B > 65535 || n_q > (1 << 24) || (double)H * B * std::max<int64_t>(1, n_q) > (double)(1 << 28)) return GGML_MI355X_EINVAL;
+    // (a grid has less than 2^32 threads: 256 for every row's join or problem, 512 for 256 rows of a prompt)
+    if (H > 65535 || B > 65535 || n_q >= (1 << 24) || H * B > (1 << 22) || H * B * n_q > (t.kp ? 1 << 25 : 1 << 28)) return GGML_MI355X_EINVAL;
     if (d.ne[0] != D || d.ne[1] != H || d.ne[2] != n_q || d.ne[3] != B) return GGML_MI355X_EINVAL;
     for (int i = 1; i < 4; ++i)
         if (d.ne[i] > 1 && d.nb[i] == 0) return GGML_MI355X_EINVAL;   // two rows in one place

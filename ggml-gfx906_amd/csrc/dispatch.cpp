@@ -627,11 +627,15 @@ int quantize(const TensorView &s, const TensorView &d, hipStream_t st) {
 // scratch: grow-only device buffer, one per (device, stream) user
 // ------------------------------------------------------------------------------------------
 void *Scratch::get(size_t bytes, hipStream_t st) {
-    if (bytes <= cap) return ptr;
+    if (bytes <= cap && (!keep || captured)) return ptr;
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(st, &cs) != hipSuccess) {
         (void)hipGetLastError();
         cs = hipStreamCaptureStatusNone;
+    }
+    if (bytes <= cap) {
+        captured = cs != hipStreamCaptureStatusNone;
+        return ptr;
     }
     if (cs != hipStreamCaptureStatusNone) {
         if (!short_in_capture)
@@ -640,13 +644,17 @@ void *Scratch::get(size_t bytes, hipStream_t st) {
         short_in_capture = true;
         return nullptr;
     }
-    if (ptr) {
+    size_t want = std::max(bytes, (size_t)1 << 20);
+    if (ptr && captured) {
+        want = std::max(want, 2 * cap);
+        kept.push_back(ptr);
+    } else if (ptr) {
         (void)hipStreamSynchronize(st);    // the only users of the old buffer are on this stream
         (void)hipFree(ptr);
-        ptr = nullptr;
-        cap = 0;
     }
-    size_t want = std::max(bytes, (size_t)1 << 20);
+    ptr = nullptr;
+    cap = 0;
+    captured = false;
     want = (want + 0xFFFFF) & ~(size_t)0xFFFFF;
     if (hipMalloc(&ptr, want) != hipSuccess) {
         (void)hipGetLastError();
@@ -683,8 +691,11 @@ int *Scratch::counters(hipStream_t st) {
 
 void Scratch::release() {
     if (ptr) (void)hipFree(ptr);
+    for (void *p : kept) (void)hipFree(p);
+    kept.clear();
     ptr = nullptr;
     cap = 0;
+    captured = false;
     ++gen;
     if (cnt) (void)hipFree(cnt);
     cnt = nullptr;
@@ -699,7 +710,10 @@ Scratch &scratch_for(hipStream_t st) {
     (void)hipGetDevice(&dev);
     std::lock_guard<std::mutex> lock(mu);
     auto &p = (*reg)[{dev, st}];
-    if (!p) p = std::make_unique<Scratch>();
+    if (!p) {
+        p = std::make_unique<Scratch>();
+        p->keep = true;
+    }
     return *p;
 }
 

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <vector>
 
 #include "../../include/ggml-mi355x.h"
 #include "qmm_args.h"
@@ -32,7 +33,9 @@ struct TensorView {
 // buffer then synchronizes the stream behind those kernels before it frees the old one.
 //
 // `gen` counts reallocations: a hipGraph captured while the buffer had generation g holds its
-// address, so the graph may be replayed only while gen is still g (backend.cpp checks it).
+// address, so the graph may be replayed only while gen is still g (backend.cpp checks it). Callers
+// without a backend object have no such check: their scratch (`keep`) leaves a buffer that a capture
+// took to that graph, and grows to twice the size, so that what is left adds up to less than what is in use.
 struct Scratch {
     std::mutex mu;
     void *ptr = nullptr;
@@ -44,6 +47,8 @@ struct Scratch {
     // itself succeeds; the backend checks this flag and runs eagerly instead (which grows the
     // buffer), so the graph it captures next holds the fast path
     bool short_in_capture = false;
+    bool keep = false, captured = false;
+    std::vector<void *> kept;
     void *get(size_t bytes, hipStream_t st);
     // stream-K tile counters (mmq8.hip): a separate zeroed allocation of COUNTERS ints, made once
     // (outside any capture) and never moved; every launch leaves them zero

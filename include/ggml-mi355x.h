@@ -181,15 +181,16 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
  * queries the weights are rounded to that type for the product with v. Results do not depend on
  * timing: every sum has a fixed order.
  *
- * D: a multiple of 8, at most 256. H, B: at most 65535; n_q: 2^24; H B n_q: 2^28. q, k, v, dst: rows
- * contiguous, data and strides multiples of 16 bytes (positions of k and v 16 MiB or more apart take a
+ * D: a multiple of 8, at most 256. H, B: at most 65535, H B 2^22; n_q: below 2^24; H B n_q: at most 2^28.
+ * q, k, v, dst: rows contiguous, data and strides multiples of 16 bytes (positions of k and v 16 MiB or more apart take a
  * slower kernel). dst must not overlap the operands. EINVAL for anything else, max_bias > 0 without a
  * mask, or parameters that are not finite or negative (scale may be negative).
  *
  * work: a workspace of ggml_mi355x_flash_attn_work_size() bytes (16-byte aligned), used only until the
  * call's kernels are done, or NULL: the library keeps one per (device, stream), which can not grow inside
  * a stream capture (ENOMEM: run the call once before capturing it) and which captured graphs of one
- * stream share: graphs that may run at the same time need workspaces of their own. */
+ * stream share: graphs that may run at the same time need workspaces of their own. A graph keeps the
+ * workspace it was captured with when a later call needs a larger one. */
 typedef struct {
     float   scale, max_bias, logit_softcap;
     int32_t causal;  /* 0 or 1 */
@@ -204,7 +205,7 @@ GGML_MI355X_API int ggml_mi355x_flash_attn_work_size(const ggml_mi355x_tensor *q
 /* ggml_mi355x_flash_attn for B sequences that share a prefix: kp, vp [D, n_prefix, Hk, 1] are read once
  * for all of them, k, v [D, n_kv, Hk, B] are each sequence's own cache behind it, and kv_len I32 [B]
  * the keys of it in use (NULL: n_kv). Every query sees the whole prefix; with causal = 1 query i sees
- * its own keys j <= kv_len - n_q + i, with 0 all kv_len. No mask, so max_bias must be 0. */
+ * its own keys j <= kv_len - n_q + i, with 0 all kv_len. No mask, so max_bias must be 0. H B n_q: at most 2^25. */
 GGML_MI355X_API int ggml_mi355x_flash_attn_prefix(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp,
                                                   const ggml_mi355x_tensor *vp, const ggml_mi355x_tensor *k,
                                                   const ggml_mi355x_tensor *v, const ggml_mi355x_tensor *sinks,

@@ -458,6 +458,38 @@ def test_callers_workspace_capture_and_replay(prefix):
 
 
 @gpu
+@pytest.mark.parametrize("small_first", [True, False])
+def test_graph_keeps_its_workspace(small_first):
+    """a call captured with the library's workspace is replayed after a later call on its stream needed a larger one"""
+    q, k, v = operands(2, 1, 4000, 8, 2, 128, "f16", "f16", seed=4)
+    big = operands(256, 4, 20, 32, 4, 128, "f16", "f16", seed=5)
+    kp, vp = rnd((8000, 4, 128), "f16", 6), rnd((8000, 4, 128), "f16", 7)
+    hf = lambda t: M.from_torch(t.permute(0, 2, 1, 3))  # noqa: E731
+    need = M.flash_attn_work_size(hf(q), hf(k))
+    assert 0 < need < 16 << 20 < M.flash_attn_prefix_work_size(hf(big[0]), M.from_torch(kp.permute(1, 0, 2)), hf(big[1]))
+    s, out = torch.cuda.Stream(), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    want = call(q, k, v, 0.09, stream=s)
+    g = torch.cuda.CUDAGraph()
+    d, spec = M.from_torch(out), M.attn_spec(0.09)
+    with torch.cuda.graph(g, stream=s):
+        M.flash_attn(hf(q), hf(k), hf(v), d, spec, stream=s)
+    if not small_first:
+        g.replay()
+        torch.cuda.synchronize()
+    large = call(*big, 0.09, kp=kp, vp=vp, stream=s)
+    assert torch.equal(large, call(*big, 0.09, kp=kp, vp=vp))
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(large, call(*big, 0.09, kp=kp, vp=vp, stream=s))
+
+
+@gpu
 def test_streams_and_threads():
     """calls on two streams, and from two host threads on one, each with the library's workspace"""
     import threading
@@ -581,6 +613,16 @@ def test_refusals(prefix):
                     dict(mask=desc(M.F16, [50, 3, 1, 4])), dict(mask=desc(M.F16, [50, 3], ptr=0)), dict(mask=desc(M.F16, [50, 3], [4, 200, 600, 600]))]
     for c in changes:
         assert rc(prefix, **c) == -1, c
+
+
+def test_refusals_of_what_no_grid_holds():
+    def of(B, n, H, Hk, D=8):
+        return dict(q=desc(M.F16, [D, n, H, B]), k=desc(M.F16, [D, 4, Hk, B]), v=desc(M.F16, [D, 4, Hk, B]), dst=desc(M.F16, [D, H, n, B]))
+
+    for sizes in ((65536, 1, 1, 1), (1, 1, 65536, 1), (1, 1 << 24, 1, 1), (65535, 1, 128, 128), (64, 1 << 18, 64, 1)):
+        assert rc(**of(*sizes)) == -1, sizes
+    pre = dict(kp=desc(M.F16, [8, 70, 2]), vp=desc(M.F16, [8, 70, 2]))
+    assert rc(True, **of(64, 1 << 14, 64, 2), **pre) == -1
 
 
 def test_workspace_sizes_and_refusals():
