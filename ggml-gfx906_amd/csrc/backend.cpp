@@ -339,6 +339,9 @@ bool attn_of(const struct ggml_tensor *node, AttnNode &a) {
     return true;
 }
 
+// a view without data yet (its buffer's begins at a large power of two): whether it will lie at a multiple of `to`
+bool view_fits(const struct ggml_tensor *t, size_t to) { return !t || t->data || !t->view_src || t->view_offs % to == 0; }
+
 // ------------------------------------------------------------------------------------------
 // buffer
 // ------------------------------------------------------------------------------------------
@@ -2159,7 +2162,8 @@ bool dv_supports_op(ggml_backend_dev_t d, const struct ggml_tensor *op) {
         }
         case GGMLABI_OP_FLASH_ATTN_EXT: {
             AttnNode a;
-            return attn_of(op, a) && check_flash_attn(a.t, a.spec) == GGML_MI355X_OK;
+            return attn_of(op, a) && view_fits(op->src[0], 16) && view_fits(op->src[1], 16) && view_fits(op->src[2], 16) && view_fits(op, 16) &&
+                   check_flash_attn(a.t, a.spec) == GGML_MI355X_OK;
         }
         default:
             break;

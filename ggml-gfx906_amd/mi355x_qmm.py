@@ -157,7 +157,27 @@ def from_torch(t) -> MmTensor:
     while len(ne) < 4:
         nb.append(nb[-1] * ne[-1] if ne else e)
         ne.append(1)
-    return tensor(kind, t.data_ptr(), ne, nb)
+    T = tensor(kind, t.data_ptr(), ne, nb)
+    T.device = t.device.index
+    return T
+
+
+_several_gpus = None
+
+
+def _on_current_gpu(*tensors) -> None:
+    """raises for descriptors (from_torch) of tensors on another GPU than the current one: a kernel runs on the
+    current one, and may not reach them"""
+    global _several_gpus
+    if _several_gpus is None:
+        import torch
+        _several_gpus = torch.cuda.device_count() > 1
+    if _several_gpus:
+        import torch
+        here = torch.cuda.current_device()
+        for t in tensors:
+            if getattr(t, "device", here) != here:
+                raise Mi355xError(f"a tensor on GPU {t.device}, the current one is {here}")
 
 
 def _stream_ptr(stream) -> int | None:
@@ -197,11 +217,13 @@ def _ref(t):
 
 def rope(src: MmTensor, pos: MmTensor, dst: MmTensor, spec: RopeSpec, factors: MmTensor = None, stream=None) -> None:
     """dst = src with its rows turned by their positions (GGML_OP_ROPE); [ne0, heads, tokens, batch]"""
+    _on_current_gpu(src, pos, dst, factors)
     _check(lib().ggml_mi355x_rope(_ref(src), _ref(pos), _ref(factors), _ref(dst), _ref(spec), _stream_ptr(stream)), "rope")
 
 
 def rope_back(src: MmTensor, pos: MmTensor, dst: MmTensor, spec: RopeSpec, factors: MmTensor = None, stream=None) -> None:
     """dst = the gradient of rope's input for src, the gradient of its result (GGML_OP_ROPE_BACK)"""
+    _on_current_gpu(src, pos, dst, factors)
     _check(lib().ggml_mi355x_rope_back(_ref(src), _ref(pos), _ref(factors), _ref(dst), _ref(spec), _stream_ptr(stream)),
            "rope_back")
 
@@ -220,6 +242,7 @@ def flash_attn(q: MmTensor, k: MmTensor, v: MmTensor, dst: MmTensor, spec: AttnS
     """dst [D, H, n_q, B] = softmax(scale q k^T + mask) v (GGML_OP_FLASH_ATTN_EXT); q [D, n_q, H, B],
     k, v [D, n_kv, Hk, Bk]; work: a tensor of flash_attn_work_size bytes"""
     p, n = _work(work)
+    _on_current_gpu(q, k, v, dst, mask, sinks, kv_len)
     _check(lib().ggml_mi355x_flash_attn(_ref(q), _ref(k), _ref(v), _ref(mask), _ref(sinks), _ref(kv_len), _ref(dst), _ref(spec),
                                         p, n, _stream_ptr(stream)), "flash_attn")
 
@@ -234,6 +257,7 @@ def flash_attn_prefix(q: MmTensor, kp: MmTensor, vp: MmTensor, k: MmTensor, v: M
                       sinks: MmTensor = None, kv_len: MmTensor = None, work=None, stream=None) -> None:
     """flash_attn of sequences behind a shared prefix kp, vp [D, n_prefix, Hk]; k, v: each one's own cache"""
     p, n = _work(work)
+    _on_current_gpu(q, kp, vp, k, v, dst, sinks, kv_len)
     _check(lib().ggml_mi355x_flash_attn_prefix(_ref(q), _ref(kp), _ref(vp), _ref(k), _ref(v), _ref(sinks), _ref(kv_len), _ref(dst),
                                                _ref(spec), p, n, _stream_ptr(stream)), "flash_attn_prefix")
 

@@ -3,6 +3,7 @@
 // on the first device. Tests load it with ctypes (RTLD_GLOBAL) before the plugin:
 //   gh_open(plugin)                                   1 when a backend came up
 //   gh_tensor(op, type, ne, nb, data, src, n_src, params, n_params) -> index of the new tensor
+//   gh_view(t, of, offset)                            t becomes a view without data yet
 //   gh_supports(t)                                    supports_op of the device
 //   gh_graph(nodes, n)  gh_compute() -> ggml_status   one graph at a time; compute waits for the result
 #include "../ggml-gfx906_amd/csrc/ggml_abi.h"
@@ -76,6 +77,12 @@ API int gh_tensor(int op, int type, const int64_t *ne, const size_t *nb, void *d
     std::memcpy(t.op_params, params, n_params * sizeof(int32_t));
     tensors.push_back(t);
     return (int)tensors.size() - 1;
+}
+
+API void gh_view(int t, int of, size_t offset) {
+    tensors[t].data = nullptr;
+    tensors[t].view_src = &tensors[of];
+    tensors[t].view_offs = offset;
 }
 
 API int gh_supports(int t) { return device->iface.supports_op(device, &tensors[t]); }

@@ -638,3 +638,18 @@ def test_workspace_sizes_and_refusals():
     assert L.ggml_mi355x_flash_attn_work_size(C.byref(q), C.byref(k), None) == -1
     assert L.ggml_mi355x_flash_attn_work_size(C.byref(q), C.byref(desc(M.F16, [64, 10, 8])), C.byref(b)) == -1
     assert L.ggml_mi355x_flash_attn_prefix_work_size(C.byref(q), None, C.byref(k), C.byref(b)) == -1
+
+
+def test_tensors_on_another_gpu_are_refused(monkeypatch):
+    monkeypatch.setattr(M, "_several_gpus", True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    a = base()
+    for name in ("q", "k", "v", "dst"):
+        x = dict(a, **{name: desc(M.F16, [64, 3, 8, 2])})
+        x[name].device = 1
+        with pytest.raises(M.Mi355xError, match="GPU 1"):
+            M.flash_attn(x["q"], x["k"], x["v"], x["dst"], x["params"], stream=0)
+        with pytest.raises(M.Mi355xError, match="GPU 1"):
+            M.flash_attn_prefix(x["q"], a["k"], a["v"], x["k"], x["v"], x["dst"], x["params"], stream=0)
+        with pytest.raises(M.Mi355xError, match="GPU 1"):
+            M.rope(x["q"], x["k"], x["v"] if name != "dst" else x["dst"], M.rope_spec(64), stream=0)

@@ -122,6 +122,18 @@ assert attn(rnd(1, 4, 3, 64), k, k) == 0
 print("REFUSED_OK", flush=True)
 '''
 
+VIEWS = BODY + r'''
+q, k = rnd(1, 4, 8, 64), rnd(1, 70, 2, 64, dtype=torch.float16)
+hf = lambda t: leaf(F(t.permute(0, 2, 1, 3)))
+whole = leaf(F(rnd(100000)))
+for of in range(3):
+    for offset, want in ((0, 1), (16, 1), (4096 + 32, 1), (8, 0), (4096 + 2, 0)):
+        src = [hf(q), hf(k), hf(k)]
+        H.gh_view(src[of], whole, C.c_size_t(offset))
+        assert H.gh_supports(node(ATTN, F(torch.empty_like(q)), src, (0.125, 0.0, 0.0, 10))) == want, (of, offset)
+print("VIEWS_OK", flush=True)
+'''
+
 
 def run(body, word):
     if not os.path.exists(HOST):
@@ -138,3 +150,9 @@ def test_graph_equals_the_direct_calls():
 @pytest.mark.gpu
 def test_supports_op_declines():
     run(REFUSED, "REFUSED_OK")
+
+
+@pytest.mark.gpu
+def test_supports_op_sees_where_a_view_will_lie():
+    """a graph is handed out before its tensors have data: a view at an odd offset is declined then, not when it runs"""
+    run(VIEWS, "VIEWS_OK")
