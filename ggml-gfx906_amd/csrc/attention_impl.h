@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // reaches 1.2). By memory where it meets few: 64 tokens, the same heads in f16, ragged to 8192 keys 295 us,
 // 5.5 TB/s; one token behind 131072 keys 101 us, 5.3. By latency in small calls: one token's 12 heads of 64
 // values, 1000 keys 6.3 us and 3.4 for the join. A mask's rows lie across a load's lanes: 16 heads of 80 values,
-// 2 x 777 queries, 1900 keys, f32, 63 us, 46 without a mask.
+// 2 x 777 queries, 1900 keys, f32, 59 us, 46 without a mask.
 // ------------------------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -670,13 +670,14 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     // whether the mask hides the tile from all of the wave's rows
     auto hidden = [&](const f16x4 (&w)[KT / 8]) {
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        if (!__all(__builtin_bit_cast(u32x2, w[0])[0] == 0xfc00fc00u)) return false;   // (most tiles end here)
         uint32_t other = 0;
 #pragma unroll
         for (int r = 0; r < KT / 8; ++r) {
             const u32x2 v = __builtin_bit_cast(u32x2, w[r]);
             other |= (v[0] ^ 0xfc00fc00u) | (v[1] ^ 0xfc00fc00u);
         }
-        return __all(other == 0);
+        return __all(other == 0) != 0;
     };
 
     // LDS reads run AHEAD operands ahead of the MFMAs that take them: left to itself the compiler, short of
@@ -841,8 +842,9 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             // this wave's share of the tile has come; behind the barrier everyone's has, and the other stage is read
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (masked) arrange(ahead, w);
-            // (8 waves that share a tile have half the DMA each, and lose 3 % by dealing it out)
-            const bool mine = j < seen_most && !(masked && hidden(w)), among = RW == 4 && mine && j + T::STEP + KT <= j_end;
+            // (8 waves that share a tile have half the DMA each, and lose 3 % by dealing it out, as do loads of a mask before
+            // it; but a wave alone on its SIMD gains 11 % with a mask too)
+            const bool mine = j < seen_most && !(masked && hidden(w)), among = RW == 4 && !(masked && DP < 256) && mine && j + T::STEP + KT <= j_end;
             if (j + T::STEP < j_end && !among) {
                 load_k(j + T::STEP, next);
                 load_v(j + T::STEP, next + BYTES);
