@@ -613,8 +613,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
         c = ldexpf(c, e2);
     }
     const bool capped = KIND != OWN && a.cap != 0.0f;
-    const float c_cap = capped ? c / a.cap : 0.0f, cap2 = a.cap * LOG2E;
-    c *= LOG2E;
+    const float cap2 = a.cap * LOG2E;
     // the maximum is taken of the bare products, so their factor must be above 0: its sign goes into
     // the queries, and for 0 a factor that leaves nothing of any product of f16 values
     if (c < 0.0f) {
@@ -625,7 +624,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             if constexpr (SPLIT) ql[t] = -ql[t];
         }
     }
-    c = fmaxf(c, 0x1p-126f);
+    const float c_cap = capped ? c / a.cap : 0.0f;
+    c = fmaxf(c * LOG2E, 0x1p-126f);
     // a mask alone joins the bare products, by the slope over their factor, where that is no extreme number
     const bool scaled = capped || (masked && __any(!(c > 0x1p-60f && c < 0x1p20f)));
     if (masked && !scaled) slope /= c;

@@ -260,6 +260,19 @@ def test_nan_and_infinity_that_a_row_sees(kv, io):
     assert ((rows.double() - o[0][keep.cuda()]).abs() <= most[0][keep.cuda()])[:, others].all()
 
 
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 9, 150])
+def test_negative_scale_under_a_cap(kv, io, n):
+    q, k, v = operands(2, n, 333, 6, 2, 64, kv, io, seed=41)
+    w = rnd((1, 1, n, 333), "f16", 42)
+    kp, vp = rnd((100, 2, 64), kv, 43), rnd((100, 2, 64), kv, 44)
+    for scale in (-0.125, -1.0):
+        near(call(q, k, v, scale, cap=7.0), formula(q, k, v, scale, full(2, 333), cap=7.0))
+        near(call(q, k, v, scale, cap=7.0, mask=w, causal=True), formula(q, k, v, scale, full(2, 333), cap=7.0, mask=w, causal=True))
+        near(call(q, k, v, scale, cap=7.0, kp=kp, vp=vp), formula(q, k, v, scale, full(2, 333), cap=7.0, kp=kp, vp=vp))
+
+
 LAUNCHES = [
     # B, n_q, n_kv, H, Hk, D: few row tiles, one for each CU, several (workgroups of 4 and 8 waves, their tiles of keys
     # shared or taken in turns, the keys split or not)
