@@ -72,7 +72,8 @@ static int check_attn(const AttnTensors &t, const AttnSpec &p) {
         if (l.type != T_I32 || l.ne[0] != B || (B > 1 && l.nb[0] % 4 != 0) || (uintptr_t)l.data % 4 != 0) return GGML_MI355X_EINVAL;
     }
     if (!std::isfinite(p.scale) || !(p.max_bias >= 0.0f) || !std::isfinite(p.max_bias) || !(p.logit_softcap >= 0.0f) ||
-        !std::isfinite(p.logit_softcap) || !(p.causal == 0 || p.causal == 1))
+        !(p.logit_softcap <= 0x1p64f) ||   // (its product with log2(e), and the scale over it, stay normal numbers)
+        !(p.causal == 0 || p.causal == 1))
         return GGML_MI355X_EINVAL;
     if (p.max_bias > 0.0f && !t.mask) return GGML_MI355X_EINVAL;   // slopes multiply a mask
     return GGML_MI355X_OK;

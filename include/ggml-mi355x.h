@@ -184,7 +184,7 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
  * D: a multiple of 8, at most 256. H, B: at most 65535, H B 2^22; n_q: below 2^24; H B n_q: at most 2^28.
  * q, k, v, dst: rows contiguous, data and strides multiples of 16 bytes (positions of k and v 16 MiB or more apart take a
  * slower kernel). dst must not overlap the operands. EINVAL for anything else, max_bias > 0 without a
- * mask, or parameters that are not finite or negative (scale may be negative).
+ * mask, logit_softcap over 2^64, or parameters that are not finite or negative (scale may be negative).
  *
  * work: a workspace of ggml_mi355x_flash_attn_work_size() bytes (16-byte aligned), used only until the
  * call's kernels are done, or NULL: the library keeps one per (device, stream), which can not grow inside

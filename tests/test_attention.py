@@ -615,7 +615,7 @@ def test_refusals(prefix):
         dict(sinks=desc(M.F32, [7])), dict(sinks=desc(M.F16, [8])), dict(kv_len=desc(M.I32, [1])), dict(kv_len=desc(M.F32, [2])),
         dict(q=desc(M.F16, [64, 3, 8, 2], ptr=0)), dict(v=desc(M.F16, [64, 50, 2, 2], ptr=0)), dict(kv_len=desc(M.I32, [2], ptr=0)), dict(sinks=desc(M.F32, [8], ptr=0)),
         dict(params=M.attn_spec(NAN)), dict(params=M.attn_spec(INF)), dict(params=M.attn_spec(1.0, -1.0)), dict(params=M.attn_spec(1.0, 8.0)),
-        dict(params=M.attn_spec(1.0, 0.0, -5.0)), dict(params=M.attn_spec(1.0, 0.0, NAN)), dict(params=M.AttnSpec(1.0, 0.0, 0.0, 2)),
+        dict(params=M.attn_spec(1.0, 0.0, -5.0)), dict(params=M.attn_spec(1.0, 0.0, NAN)), dict(params=M.attn_spec(1.0, 0.0, INF)), dict(params=M.attn_spec(1.0, 0.0, 1e20)), dict(params=M.AttnSpec(1.0, 0.0, 0.0, 2)),
         dict(q=None), dict(k=None), dict(v=None), dict(dst=None), dict(params=None),
     ]
     if prefix:
