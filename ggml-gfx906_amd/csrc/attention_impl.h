@@ -82,6 +82,11 @@ __device__ void row_keys(const AttnArgs &a, const float (&q)[4], const char *k, 
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             if (lane + 64 * c < a.D) r.o[c] = r.o[c] * f + p * (float)vr[lane + 64 * c];
+        // a row that is NaN throughout stays it: NaN weights of a whole model must not cost every key for every row
+        bool lost = true;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) lost &= lane + 64 * c >= a.D || r.o[c] != r.o[c];
+        if (__all(lost)) return;
     }
 }
 

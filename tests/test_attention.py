@@ -317,6 +317,28 @@ def test_masks_beside_extreme_scales(kv, io, scale):
 
 @gpu
 @pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 7, 1500])
+@pytest.mark.parametrize("what", ["q", "k", "v", "all"])
+def test_nan_throughout(kv, io, n, what):
+    """rows that see NaN only, or behind the second key, are NaN; rows that see none of it are what they are"""
+    q, k, v = operands(2, n, 1600, 8, 2, 128, kv, io, seed=n)
+    kp, vp = rnd((300, 2, 128), kv, 51), rnd((300, 2, 128), kv, 52)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if what in (name, "all"):
+            t[:] = NAN
+    assert torch.isnan(call(q, k, v, 0.09)).all() and torch.isnan(call(q, k, v, 0.09, kp=kp, vp=vp)).all()
+    if what in ("k", "v"):
+        q, k, v = operands(2, n, 1600, 8, 2, 128, kv, io, seed=n)
+        (k if what == "k" else v)[:, 2:] = NAN
+        lens = ints(1600, min(2, n))
+        got = call(q, k, v, 0.09, lens, causal=True)
+        assert torch.isnan(got[0]).all()
+        o, most, _ = formula(q, k[:, :2], v[:, :2], 0.09, ints(2, min(2, n)), causal=True)
+        assert ((got[1].double() - o[1]).abs() <= most[1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
 @pytest.mark.parametrize("n", [1, 50])
 def test_cap_sinks_and_large_scores(kv, io, n):
     q, k, v = operands(2, n, 150, 8, 2, 64, kv, io, seed=21)
