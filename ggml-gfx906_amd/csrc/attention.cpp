@@ -141,6 +141,7 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     };
     auto join = [&](int slots) { return slots > 1 ? 5.0 + (double)B * H * n_q * slots * D * 8 / 5e6 : 0.0; };
     static const int SPLITS[] = {1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 28, 32, 48, 64, 96, 128};
+    static const int PREFIX_SPLITS[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 18, 20, 22, 24, 26, 28, 30, 32, 48, 64, 96, 128};
     static_assert(128 <= ATTN_MAX_SLOTS / 2, "a prefix's splits and the batches' own");
     p.own_rows = rows > 32;
     p.pre_rows = t.kp && B * rows > 32;
@@ -153,25 +154,37 @@ static AttnPlan plan_attn(const AttnTensors &t) {
         const bool wide = w.waves == 8;
         if (wide && (!p.own_rows || D > 128)) continue;
         if (t.kp && (w.turns > 1 || (p.own_rows && D <= 128 && !wide))) continue;
-        for (int so : SPLITS) {
-            if (so > 1 && ((so - 1) * 32 >= n_kv || (t.kp && so > 4))) break;
+        auto consider = [&](int so, int sp) {
+            if ((so > 1 && (so - 1) * 32 >= n_kv) || (sp > 1 && (sp - 1) * 32 >= n_pre)) return false;
             const Part own = part(rows, B * Hk, n_kv, p.own_rows, w.waves, w.turns, so);
-            for (int sp : SPLITS) {
-                if (sp > 1 && (sp - 1) * 32 >= n_pre) break;
-                const Part pre = t.kp ? part(B * rows, Hk, n_pre, p.pre_rows, w.waves, 1, sp) : Part{};
-                const int slots = t.kp ? so + sp : so;
-                const double us = launch(pre, own, w.waves) + join(slots);
-                if (p.slots != 0 && us >= best) continue;
-                best = us;
-                p.waves = w.waves;
-                p.turns = w.turns;
-                p.own_splits = so;
-                p.own_tiles = own.tiles;
-                p.pre_splits = t.kp ? sp : 0;
-                p.pre_tiles = pre.tiles;
-                p.slots = slots;
-            }
+            const Part pre = t.kp ? part(B * rows, Hk, n_pre, p.pre_rows, w.waves, 1, sp) : Part{};
+            const double us = launch(pre, own, w.waves) + join(so + sp);
+            if (p.slots != 0 && us >= best) return true;
+            best = us;
+            p.waves = w.waves;
+            p.turns = w.turns;
+            p.own_splits = so;
+            p.own_tiles = own.tiles;
+            p.pre_splits = sp;
+            p.pre_tiles = pre.tiles;
+            p.slots = so + sp;
+            return true;
+        };
+        if (!t.kp) {
+            for (int so : SPLITS)
+                if (!consider(so, 0)) break;
+            continue;
         }
+        // the prefix's splits, then the own keys', and the prefix's again beside those
+        for (int sp : PREFIX_SPLITS)
+            if (!consider(1, sp)) break;
+        const int sp = p.pre_splits;
+        for (int so : SPLITS)
+            if (so > 1 && !consider(so, sp)) break;
+        if (p.own_splits == 1) continue;
+        const int so = p.own_splits;
+        for (int again : PREFIX_SPLITS)
+            if (!consider(so, again)) break;
     }
     return p;
 }

@@ -403,6 +403,7 @@ PREFIXES = [
     (1, 1, 1, 1, 1, 1, 64), (3, 1, 500, 60, 12, 12, 64), (2, 1, 0, 50, 8, 2, 128), (5, 1, 33, 1, 8, 1, 128), (64, 1, 300, 40, 8, 2, 128),
     (4, 4, 1000, 70, 32, 4, 128), (2, 3, 64, 3, 7, 1, 80), (17, 1, 129, 31, 16, 4, 256), (1, 8, 4100, 20, 8, 2, 64), (9, 2, 257, 300, 14, 2, 96),
     (40, 1, 2000, 100, 32, 8, 64), (3, 40, 200, 50, 4, 2, 128), (130, 1, 70, 5, 1, 1, 64),
+    (1, 1, 40, 9000, 8, 2, 128), (2, 3, 700, 5000, 8, 1, 64), (1, 50, 300, 4000, 8, 2, 128),   # long caches behind the prefix
 ]
 
 
