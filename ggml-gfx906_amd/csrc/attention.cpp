@@ -106,7 +106,8 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     // causal heads of 8192 tokens 547, 533, 588 / 526, 510, 557; of 2048 60, 61, 50 / 71, 70, 41; 16 of 512 behind 512
     // 27.9, 33.2, 22.8 / 29, 40, 23, the latter's 2 and 4 splits 23.9, 24.9 / 24, 23.
     const int64_t D = t.q.ne[0], rows = n_q * G;
-    const double size = t.q.type == T_F32 ? 1.8 : 1.0, size4 = size * (D <= 64 ? 0.55 : D <= 96 ? 0.83 : 1.0), size8 = size * (D <= 64 ? 0.65 : D <= 96 ? 0.83 : 1.0);
+    const double size = t.q.type == T_F32 ? 1.8 : 1.0, size4 = size * (D <= 64 ? 0.55 : D <= 96 ? 0.83 : D <= 128 || D > 192 ? 1.0 : 0.75),
+                 size8 = size * (D <= 64 ? 0.65 : D <= 96 ? 0.83 : 1.0);
     // workgroups, us of each alone on its CU and not, bytes of split keys
     struct Part { double groups, alone, beside, bytes; int tiles; };
     auto part = [&](int64_t rows, int64_t problems, int64_t keys, bool by_rows, int waves, int turns, int s) {
@@ -120,7 +121,9 @@ static AttnPlan plan_attn(const AttnTensors &t) {
     };
     const double fewer = t.k.ne[1] > 0 ? std::min(1.0, (double)n_q / (double)t.k.ne[1]) : 0.0;   // of the first rows, causal
     auto launch = [&](const Part &pre, const Part &own, int waves) {
-        const double at_once = D > 128 || waves == 8 ? 256.0 : 512.0, all = pre.groups + own.groups;
+        // (over 128 values: split keys' LDS, over 192 and f32 ones the accumulators leave room for one)
+        const bool one = waves == 8 || D > 192 || (D > 128 && (!p.own_rows || t.q.type == T_F32));
+        const double at_once = one ? 256.0 : 512.0, all = pre.groups + own.groups;
         auto us = [&](const Part &x) { return x.bytes == 0.0 && all > 256.0 ? x.beside : x.alone; };
         const double own_us = us(own), pre_us = us(pre);
         // what split keys draw from memory, beside the time that row tiles hold the CUs
@@ -255,11 +258,11 @@ int flash_attn(const AttnTensors &t, const AttnSpec &p, void *work, hipStream_t 
     }
     const AttnPlan pl = plan_attn(t);
     typedef hipError_t (*Launch)(const AttnArgs &, const AttnPlan &, void *, hipStream_t);
-    static const Launch launch[3][4] = {{attn_launch_f16_64, attn_launch_f16_96, attn_launch_f16_128, attn_launch_f16_256},
-                                        {attn_launch_bf16_64, attn_launch_bf16_96, attn_launch_bf16_128, attn_launch_bf16_256},
-                                        {attn_launch_f32_64, attn_launch_f32_96, attn_launch_f32_128, attn_launch_f32_256}};
+    static const Launch launch[3][5] = {{attn_launch_f16_64, attn_launch_f16_96, attn_launch_f16_128, attn_launch_f16_192, attn_launch_f16_256},
+                                        {attn_launch_bf16_64, attn_launch_bf16_96, attn_launch_bf16_128, attn_launch_bf16_192, attn_launch_bf16_256},
+                                        {attn_launch_f32_64, attn_launch_f32_96, attn_launch_f32_128, attn_launch_f32_192, attn_launch_f32_256}};
     const int type = q.type == T_F32 ? 2 : q.type == T_BF16 ? 1 : 0;
-    const hipError_t e = launch[type][a.D <= 64 ? 0 : a.D <= 96 ? 1 : a.D <= 128 ? 2 : 3](a, pl, work, st);
+    const hipError_t e = launch[type][a.D <= 64 ? 0 : a.D <= 96 ? 1 : a.D <= 128 ? 2 : a.D <= 192 ? 3 : 4](a, pl, work, st);
     return e == hipSuccess ? GGML_MI355X_OK : GGML_MI355X_EHIP;
 }
 

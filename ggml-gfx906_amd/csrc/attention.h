@@ -52,14 +52,17 @@ struct AttnPlan {
 ATTN_LAUNCH(attn_launch_f16_64)
 ATTN_LAUNCH(attn_launch_f16_96)
 ATTN_LAUNCH(attn_launch_f16_128)
+ATTN_LAUNCH(attn_launch_f16_192)
 ATTN_LAUNCH(attn_launch_f16_256)
 ATTN_LAUNCH(attn_launch_bf16_64)
 ATTN_LAUNCH(attn_launch_bf16_96)
 ATTN_LAUNCH(attn_launch_bf16_128)
+ATTN_LAUNCH(attn_launch_bf16_192)
 ATTN_LAUNCH(attn_launch_bf16_256)
 ATTN_LAUNCH(attn_launch_f32_64)
 ATTN_LAUNCH(attn_launch_f32_96)
 ATTN_LAUNCH(attn_launch_f32_128)
+ATTN_LAUNCH(attn_launch_f32_192)
 ATTN_LAUNCH(attn_launch_f32_256)
 #undef ATTN_LAUNCH
 

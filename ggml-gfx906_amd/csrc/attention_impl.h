@@ -959,7 +959,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 // in LDS: half the splits, or none, where row tiles are few. 4 where the largest heads' accumulators leave room for
 // no more. Causal heads of 128 values, 32 on 8, 2048 tokens: 60 us by 4 waves, 61 by 8, 50 in turns; 8192: 547, 533, 588.
 template <typename TK, typename TQ, int DC, int WAVES, int PRE, bool OWN_ROWS, bool GENERAL, int TURNS>
-__global__ __launch_bounds__(WAVES * 64, DC == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
+__global__ __launch_bounds__(WAVES * 64, DC == 256 || (DC == 192 && sizeof(TQ) == 4) ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnPart pre, const AttnPart own) {
     constexpr int L0 = AttnTile<TK, TQ, DC, WAVES, OWN_ROWS, TURNS>::LDS, L1 = AttnTile<TK, TQ, DC, WAVES, PRE == 2>::LDS;
     __shared__ __align__(16) char lds[PRE && L1 > L0 ? L1 : L0];
     if constexpr (PRE != 0) {

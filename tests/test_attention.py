@@ -278,6 +278,7 @@ LAUNCHES = [
     # shared or taken in turns, the keys split or not)
     (1, 300, 3000, 8, 2, 64), (1, 515, 1031, 16, 4, 128), (1, 300, 1500, 32, 8, 96), (1, 1024, 1030, 32, 8, 128), (1, 2049, 2049, 16, 8, 88),
     (2, 2048, 2050, 32, 4, 64), (2, 2048, 2048, 32, 4, 128), (4, 700, 900, 32, 8, 96), (2, 777, 1900, 16, 16, 80), (1, 600, 1000, 16, 2, 256),
+    (1, 1000, 1500, 32, 8, 160), (2, 1500, 1500, 16, 16, 192), (3, 5, 900, 16, 2, 136),
 ]
 
 
@@ -403,7 +404,7 @@ PREFIXES = [
     (1, 1, 1, 1, 1, 1, 64), (3, 1, 500, 60, 12, 12, 64), (2, 1, 0, 50, 8, 2, 128), (5, 1, 33, 1, 8, 1, 128), (64, 1, 300, 40, 8, 2, 128),
     (4, 4, 1000, 70, 32, 4, 128), (2, 3, 64, 3, 7, 1, 80), (17, 1, 129, 31, 16, 4, 256), (1, 8, 4100, 20, 8, 2, 64), (9, 2, 257, 300, 14, 2, 96),
     (40, 1, 2000, 100, 32, 8, 64), (3, 40, 200, 50, 4, 2, 128), (130, 1, 70, 5, 1, 1, 64),
-    (1, 1, 40, 9000, 8, 2, 128), (2, 3, 700, 5000, 8, 1, 64), (1, 50, 300, 4000, 8, 2, 128),   # long caches behind the prefix
+    (1, 1, 40, 9000, 8, 2, 128), (2, 3, 700, 5000, 8, 1, 64), (1, 50, 300, 4000, 8, 2, 128), (57, 3, 700, 20, 21, 3, 144), (4, 20, 500, 90, 8, 2, 192),   # long caches behind the prefix
 ]
 
 
