@@ -156,7 +156,7 @@ int check_rope(const TensorView &src, const TensorView &pos, const TensorView *f
 int rope(const TensorView &src, const TensorView &pos, const TensorView *ff, const TensorView &dst, const RopeSpec &p, bool back,
          hipStream_t st);
 
-// attention over a key / value cache (attention.hip); kp / vp: a prefix that every batch shares
+// attention over a key / value cache (attention.cpp); kp / vp: a prefix that every batch shares
 typedef ggml_mi355x_attn_params AttnSpec;
 struct AttnTensors {
     TensorView q, k, v, dst;
