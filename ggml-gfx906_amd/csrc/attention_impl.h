@@ -151,8 +151,9 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // twice; the DMA writes LDS in order, so the permutation is in the addresses it reads from.
 //
 // m moves only when a tile exceeds it by more than 2^LAZY, so the 16 DP/32 accumulators are rarely
-// rescaled; weights are kept 2^BIAS times larger, up to 2^(BIAS + LAZY) = 2^15, which f16 still holds, so
-// that small ones stay clear of f16's subnormals.
+// rescaled; weights are kept 2^BIAS times larger: f16 ones up to 2^(BIAS + LAZY) = 2^15, which f16 still holds,
+// so that small ones stay clear of its subnormals (f16 values times them stay far below f32's end); bf16 ones
+// up to 1, since a bf16 value may lie anywhere in f32's range and its product must too.
 // F32 queries: q (scaled by a power of two per row) and p are each carried as a sum of two f16 values
 // (2^-22), two MFMAs per product.
 //
@@ -173,11 +174,17 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(3))) char *lds_const;
 
-constexpr float BIAS = 8.0f, LAZY = 7.0f;
+constexpr float LAZY = 7.0f;
 
 template <typename T> struct Vec;
-template <> struct Vec<_Float16> { typedef f16x8 x8; };
-template <> struct Vec<__bf16> { typedef bf16x8 x8; };
+template <> struct Vec<_Float16> {
+    typedef f16x8 x8;
+    static constexpr float BIAS = 8.0f;
+};
+template <> struct Vec<__bf16> {
+    typedef bf16x8 x8;
+    static constexpr float BIAS = -LAZY;
+};
 
 __device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -493,6 +500,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     using T = AttnTile<TK, TQ, DC, WAVES, BY_ROWS, TURNS>;
     typedef typename T::x8 x8;
     constexpr bool SPLIT = T::SPLIT, PREFIX = KIND == PREFIX_KEYS;
+    constexpr float BIAS = Vec<TK>::BIAS;
     constexpr int DP = T::DP, KT = T::KT, CPR = T::CPR, RPD = T::RPD, ROUNDS = T::ROUNDS, BYTES = T::BYTES, NT = DC / 16, NB = DC / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     // problem, row tile (the last ones first: with a causal rule they see the most keys), split of the keys
