@@ -154,8 +154,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // rescaled; weights are kept 2^BIAS times larger: f16 ones up to 2^(BIAS + LAZY) = 2^15, which f16 still holds,
 // so that small ones stay clear of its subnormals (f16 values times them stay far below f32's end); bf16 ones
 // up to 1, since a bf16 value may lie anywhere in f32's range and its product must too.
-// F32 queries: q (scaled by a power of two per row) and p are each carried as a sum of two f16 values
-// (2^-22), two MFMAs per product.
+// F32 queries: q (scaled by a power of two per row) and p are each carried as a sum of two f16 values, two MFMAs per
+// product: to 2^-22 of the value, or of q 2^-40 of its row's largest, of p 2^-33 of the largest weight.
 //
 // Bound by the matrix cores and, beside them, the vector units' exponentials, maxima and sums where a key
 // meets many rows: 8192 causal tokens, 32 heads on 8 of 128 bf16 values 528 us, 1.04 PFLOP/s (a large library product
@@ -605,25 +605,29 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 
     float c = a.scale;
     if constexpr (SPLIT) {
+        // (infinities are no measure of the others, and have no second term)
         float top = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(qx[t][e]));
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(qx[t][e]) < INFINITY ? fabsf(qx[t][e]) : 0.0f);
         top = fmaxf(top, swap32_f(top));
-        // 2^-e * q below 1: no f16 overflows, and the second term keeps its bits
-        int e2 = 0;
-        if (top > 0.0f && top < INFINITY) (void)frexpf(top, &e2);
+        // 2^up * q below 2^15: no f16 overflows, and the second term lies as far above f16's subnormals as it can
+        int up = 0;
+        if (top > 0.0f) {
+            (void)frexpf(top, &up);
+            up = 15 - up;
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = ldexpf(qx[2 * t + e / 4][e % 4], -e2);
+                const float x = ldexpf(qx[2 * t + e / 4][e % 4], up);
                 const _Float16 hi = (_Float16)x;
                 qf[t][e] = hi;
-                ql[t][e] = (_Float16)(x - (float)hi);
+                ql[t][e] = fabsf(x) < INFINITY ? (_Float16)(x - (float)hi) : (_Float16)0.0f;
             }
-        c = ldexpf(c, e2);
+        c = ldexpf(c, -up);
     }
     const bool capped = KIND != OWN && a.cap != 0.0f;
     const float cap2 = a.cap * LOG2E;

@@ -177,7 +177,8 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
  * causal: the queries are the last n_q of the keys in use, query i sees keys j <= kv_len - n_q + i
  * (with a mask as well: both hold). Keys that a row does not see take no part in it, whatever their
  * bytes hold; rows that see no key are zeros. logit_softcap c > 0: scaled scores become
- * c tanh(score / c) before the mask. F32 queries and weights keep 32-bit accuracy; with F16 / BF16
+ * c tanh(score / c) before the mask. F32 queries and their weights are each taken as a sum of two F16 terms, exact
+ * to 2^-22 of the value (or 2^-40 of the row's largest query value, 2^-33 of its largest weight); with F16 / BF16
  * queries the weights are rounded to that type for the product with v. Results do not depend on
  * timing: every sum has a fixed order.
  *

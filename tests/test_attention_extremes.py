@@ -3,7 +3,7 @@ out what a row does not see."""
 import math
 
 import pytest
-from test_attention import IDS, PAIRS, TYPES, call, formula, full, near, operands, rnd, torch
+from test_attention import IDS, INF, PAIRS, TYPES, call, formula, full, near, operands, rnd, torch
 
 gpu = pytest.mark.gpu
 
@@ -43,3 +43,56 @@ def test_largest_values(kv, io, n, D):
     k3[..., 0], k3[:, 0, :, 0], k3[:, 400, :, 0] = -30.0 / 4, 0.0, 4.5 / 4
     v3[:, 400], v3[:, 0] = large, large / 2
     near(call(q2, k3, v3, 1.0), formula(q2, k3, v3, 1.0, full(1, m)))
+
+
+# ---- f32 queries -------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 5, 70, 600])
+@pytest.mark.parametrize("D", [64, 80, 128, 192, 256])
+@pytest.mark.parametrize("size", [30.0, 1000.0, 16384.0, -3.0e6])
+def test_queries_with_one_large_value(n, D, size):
+    """f32 queries with one value far above the rest over keys that hold next to nothing there: the rest keep their
+    precision"""
+    m = 300
+    q, k, v = operands(2, n, m, 8, 2, D, "f16", "f32", seed=n + D)
+    kp, vp = rnd((100, 2, D), "f16", 7), rnd((100, 2, D), "f16", 8)
+    w = rnd((1, 1, n, m), "f16", 9)
+    w[..., 1::7] = -INF
+    q[..., 3] = size
+    s = 1 / math.sqrt(D)
+    for small in (0.0, 0.5 / abs(size)):
+        k[..., 3], kp[..., 3] = small, small
+        near(call(q, k, v, s), formula(q, k, v, s, full(2, m)))
+        near(call(q, k, v, -s, causal=True), formula(q, k, v, -s, full(2, m), causal=True))
+        near(call(q, k, v, s, mask=w, bias=8.0), formula(q, k, v, s, full(2, m), mask=w, bias=8.0))
+        near(call(q, k, v, s, cap=5.0, kp=kp, vp=vp), formula(q, k, v, s, full(2, m), cap=5.0, kp=kp, vp=vp))
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("beside", [1.0, 3.0e4, 1.0e6])
+def test_infinite_queries_under_a_cap(kv, io, n, beside):
+    """a query value of infinity makes scores of infinity, whatever is beside it, and the cap makes them finite"""
+    if beside > torch.finfo(TYPES[io]).max:
+        beside = torch.finfo(TYPES[io]).max
+    m, D, i, cap = 200, 64, n // 2, 3.0
+    q, k, v = operands(1, n, m, 4, 2, D, kv, io, seed=3)
+    q[..., 5] = beside
+    k[..., 2] = torch.where(k[..., 2].abs() < 0.1, 0.5, k[..., 2].float()).to(k.dtype)
+    q2 = q.clone()
+    q2[0, i, 1, 2] = INF
+    got = call(q2, k, v, 0.125, cap=cap)
+    # its row: weights of 1 and e^-6, by the key's sign there; every other row as without it
+    p = torch.exp(cap * torch.sign(k[0, :, 0, 2].double()) - cap)
+    row = (p[:, None] * v[0, :, 0].double()).sum(0) / p.sum()
+    A = (p[:, None] * v[0, :, 0].double().abs()).sum(0) / p.sum()
+    eps = 0.0 if io == "f32" else torch.finfo(TYPES[io]).eps / 2
+    allowed = ((2 * 6 * cap + 8 + m) * 2.0**-24 + 2 * eps) * A
+    assert ((got[0, i, 1].double() - row).abs() <= allowed).all()
+    o, most, _ = formula(q, k, v, 0.125, full(1, m), cap=cap)
+    fine = (got.double() - o).abs() <= most
+    fine[0, i, 1] = True
+    assert fine.all()
