@@ -12,6 +12,8 @@
 #include "attention.h"
 #include "qcommon.h"
 
+#include <type_traits>
+
 namespace mi355x {
 
 namespace {
@@ -632,13 +634,24 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     const bool capped = KIND != OWN && a.cap != 0.0f;
     const float cap2 = a.cap * LOG2E;
     // the maximum is taken of the bare products, so their factor must be above 0: its sign goes into
-    // the queries, and for 0 a factor that leaves nothing of any product of f16 values
+    // the queries, and for 0 a factor that leaves nothing of any product
     if (c < 0.0f) {
         c = -c;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             qf[t] = -qf[t];
             if constexpr (SPLIT) ql[t] = -ql[t];
+        }
+    }
+    if constexpr (std::is_same<TK, __bf16>::value) {
+        // (bf16 products reach 2^128: beside such a factor 2^64 of it goes over to it; a query that this brings below
+        // bf16's range is below 2^-62, and its products times the factor below 2^-34)
+        if (c < 0x1p-100f) {
+            c *= 0x1p64f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[t][e] = (TK)((float)qf[t][e] * 0x1p-64f);
         }
     }
     const float c_cap = capped ? c / a.cap : 0.0f;

@@ -96,3 +96,23 @@ def test_infinite_queries_under_a_cap(kv, io, n, beside):
     fine = (got.double() - o).abs() <= most
     fine[0, i, 1] = True
     assert fine.all()
+
+
+# ---- factors of nothing ------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("scale", [0.0, 1.0e-40, -1.0e-38])
+def test_next_to_no_factor_beside_large_products(kv, io, n, scale):
+    """bf16 products reach 1e38, where even the smallest factor counts and a factor of 0 still leaves nothing"""
+    size = 1.0e18 if kv == "bf16" else 100.0
+    q, k, v = operands(2, n, 150, 4, 2, 64, kv, io, seed=11)
+    q, k = q * size, k * size
+    w = rnd((1, 1, n, 150), "f16", 12)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    kp, vp = rnd((100, 2, 64), kv, 7) * size, rnd((100, 2, 64), kv, 8)
+    near(call(q, k, v, scale), formula(q, k, v, scale, full(2, 150)))
+    near(call(q, k, v, scale, mask=w), formula(q, k, v, scale, full(2, 150), mask=w))
+    near(call(q, k, v, scale, kp=kp, vp=vp), formula(q, k, v, scale, full(2, 150), kp=kp, vp=vp))
