@@ -254,6 +254,21 @@ struct AttnTile {
     typedef typename Vec<TK>::x8 x8;
 };
 
+// F32 queries as two f16 terms. A row is scaled to below 2^15, so that no f16 overflows and the second terms lie as far
+// above f16's subnormals as they can; infinities are no measure of the others, and have no second term
+__device__ __forceinline__ float size_of(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
+__device__ __forceinline__ int shift_of(float top) {
+    if (top == 0.0f) return 0;
+    int e;
+    (void)frexpf(top, &e);
+    return 15 - e;
+}
+__device__ __forceinline__ void query_terms(float q, int up, _Float16 &hi, _Float16 &lo) {
+    const float x = ldexpf(q, up);
+    hi = (_Float16)x;
+    lo = fabsf(x) < INFINITY ? (_Float16)(x - (float)hi) : (_Float16)0.0f;
+}
+
 // a finished row's place: the call's result, or this launch's partial result (sum, maximum, weighted values)
 struct RowOut {
     int b, i, head;
@@ -283,45 +298,6 @@ __device__ __forceinline__ float finish(const AttnArgs &a, int head, float m, fl
     return l == 0.0f ? 0.0f : f / l;
 }
 
-// A weight of 0 times a NaN or an infinity in a key that a row does not see, but another row of its tile
-// or the DMA's filling does, makes the row's sums NaN. Such a row is done again by its wave, key by key,
-// without the keys that it does not see; a NaN that it does see comes out again.
-template <typename TK, typename TQ, bool PREFIX>
-__device__ void redo_row(const AttnArgs &a, const AttnPart &p, int row, int bh, int split, int j_begin, int j_end) {
-    const int lane = threadIdx.x & 63;
-    const RowOut w = row_out<PREFIX>(a, p, row, bh, split);
-    const int pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk, bk = PREFIX ? 0 : a.by_kv_b.of(pb);
-    float q[4];
-    const TQ *qr = reinterpret_cast<const TQ *>(a.q + w.i * a.q_i + w.head * a.q_h + w.b * a.q_b);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) q[c] = lane + 64 * c < a.D ? (float)qr[lane + 64 * c] : 0.0f;
-    RowState r{-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
-    if constexpr (PREFIX) {
-        row_keys<TQ, TK>(a, q, a.kp + hk * a.kp_h, a.kp_j, a.vp + hk * a.vp_h, a.vp_j, nullptr, 0.0f, j_begin, j_end, 1, r);
-    } else {
-        const int seen = a.causal ? own_len(a, w.b) - a.n_q + w.i + 1 : j_end;
-        const _Float16 *mask = nullptr;
-        if (a.mask) mask = reinterpret_cast<const _Float16 *>(a.mask + w.i * a.m_i + (w.head % a.m_nh) * a.m_h + (w.b % a.m_nb) * a.m_b);
-        row_keys<TQ, TK>(a, q, a.k + hk * a.k_h + bk * a.k_b, a.k_j, a.v + hk * a.v_h + bk * a.v_b, a.v_j, mask, slope_of(a, w.head), j_begin,
-                         min(j_end, seen), 1, r);
-    }
-    if (p.part_o) {
-        if (lane == 0) {
-            p.part_ml[2 * w.slot] = r.m;
-            p.part_ml[2 * w.slot + 1] = r.l;
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < a.D) p.part_o[w.slot * a.D + lane + 64 * c] = r.o[c];
-    } else {
-        const float f = finish(a, w.head, r.m, r.l);
-        TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < a.D) out[lane + 64 * c] = (TQ)(r.o[c] * f);
-    }
-}
-
 template <typename TQ> __device__ __forceinline__ void store4(TQ *p, f32x4 x);
 template <> __device__ __forceinline__ void store4(float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; }
 template <> __device__ __forceinline__ void store4(_Float16 *p, f32x4 x) {
@@ -331,12 +307,161 @@ template <> __device__ __forceinline__ void store4(__bf16 *p, f32x4 x) {
     *reinterpret_cast<bf16x4 *>(p) = bf16x4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
 }
 
-// a wave's 32 rows out of the accumulators: lane (row, h) holds values 32 d + 8 r4 + 4 h .. + 3
+// a row out of the accumulators: lane (row, h) holds values 32 d + 8 r4 + 4 h .. + 3
+template <typename TQ, int NB>
+__device__ __forceinline__ void put_row(const AttnArgs &a, const AttnPart &p, const RowOut &w, const f32x16 (&o)[NB], float m, float l) {
+    const int h = (threadIdx.x & 63) >> 5;
+    if (p.part_o && h == 0) {
+        p.part_ml[2 * w.slot] = m;
+        p.part_ml[2 * w.slot + 1] = l;
+    }
+    const float f = p.part_o ? 1.0f : finish(a, w.head, m, l);
+    float *po = p.part_o + w.slot * a.D;
+    TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            if (32 * d + 8 * r4 >= a.D) continue;   // (D is a multiple of 8)
+            const int at = 32 * d + 8 * r4 + 4 * h;
+            const f32x4 x = f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]} * f;
+            if (p.part_o) *reinterpret_cast<f32x4 *>(po + at) = x;
+            else store4<TQ>(out + at, x);
+        }
+}
+
+// A weight of 0 times a NaN or an infinity in a key that a row does not see, but another row of its tile
+// or the DMA's filling does, makes the row's sums NaN. Such rows (bits of `again`) are formed again by a wave, all at
+// once: the scores of 32 keys by the same products, out of operands read straight from memory, then the keys' values one
+// key at a time, for the rows that see it; a NaN that a row does see comes out again. It ends where the weights of all rows
+// have become NaN, which makes them NaN throughout. Rolled loops and few registers, so that the tiles' loop,
+// which nearly always is all there is, keeps its own (values by MFMA out of unrolled loads held 200 more scalars and cost
+// 64-value heads a wave a SIMD). Bound by the vector units and the loads' latency, 0.8 us a key: 8192 causal tokens, 32
+// heads on 8 of 128 bf16 values, 0.54 ms, with one NaN value that every row sees 17 (500 a row and a key at a
+// time); 2048 masked f32 queries 0.12, with a NaN in one hidden key 2.0.
 template <typename TK, typename TQ, int DC, bool PREFIX>
-__device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DC / 32], float m, float l, int row,
+__device__ __forceinline__ void redo_rows(const AttnArgs &a, const AttnPart &p, int row0, uint32_t again, int bh, int split, int j_begin, int j_end) {
+    typedef typename Vec<TK>::x8 x8;
+    constexpr bool SPLIT = sizeof(TQ) == 4;
+    constexpr int NT = DC / 16, NB = DC / 32;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // (or the compiler keeps the caller's addresses of the row through its loop)
+    const int h = lane >> 5;
+    const RowOut w = row_out<PREFIX>(a, p, min(row0 + (lane & 31), p.rows - 1), bh, split);
+    const int pb = a.by_Hk.of(bh), hk = bh - pb * a.Hk, bk = PREFIX ? 0 : a.by_kv_b.of(pb);
+    const char *kb = PREFIX ? a.kp + hk * a.kp_h : a.k + hk * a.k_h + bk * a.k_b;
+    const char *vb = PREFIX ? a.vp + hk * a.vp_h : a.v + hk * a.v_h + bk * a.v_b;
+    const int64_t k_j = PREFIX ? a.kp_j : a.k_j, v_j = PREFIX ? a.vp_j : a.v_j;
+    const int seen = min(j_end, PREFIX ? a.n_prefix : a.causal ? own_len(a, w.b) - a.n_q + w.i + 1 : own_len(a, w.b));
+    const _Float16 *mask = nullptr;
+    if (!PREFIX && a.mask) mask = reinterpret_cast<const _Float16 *>(a.mask + w.i * a.m_i + (w.head % a.m_nh) * a.m_h + (w.b % a.m_nb) * a.m_b);
+    const float slope = mask ? slope_of(a, w.head) * LOG2E : 0.0f;
+    const TQ *q = reinterpret_cast<const TQ *>(a.q + w.i * a.q_i + w.head * a.q_h + w.b * a.q_b);
+    int up = 0;
+    if constexpr (SPLIT) {
+        float size = 0.0f;
+        for (int d = 0; d < a.D; ++d) size = fmaxf(size, size_of(q[d]));
+        up = shift_of(size);
+    }
+    const float c = ldexpf(a.scale, -up);
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int d = 0; d < NB; ++d) o[d] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    for (int j = j_begin; j < j_end && __any(j < seen); j += 32) {
+        f32x16 s{};
+        const TK *kr = reinterpret_cast<const TK *>(kb + min(j + (lane & 31), j_end - 1) * k_j);
+#pragma unroll 2
+        for (int t = 0; t < NT; ++t) {
+            const int d = 16 * t + 8 * h;
+            x8 kf{}, qf{}, ql{};
+            if (d < a.D) {
+                kf = *reinterpret_cast<const x8 *>(kr + d);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        _Float16 hi, lo;
+                        query_terms(q[d + e], up, hi, lo);
+                        qf[e] = hi;
+                        ql[e] = lo;
+                    }
+                } else {
+                    qf = *reinterpret_cast<const x8 *>(q + d);
+                }
+            }
+            s = mma(kf, qf, s);
+            if constexpr (SPLIT) s = mma(kf, ql, s);
+        }
+        // s[r] belongs to key j + 8 (r / 4) + 4 h + r % 4
+        uint32_t sees = 0;
+        float top = m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int key = j + 8 * (r / 4) + 4 * h + r % 4;
+            bool see = key < seen;
+            float x = s[r] * c;
+            if (a.cap != 0.0f) x = a.cap * tanh_of(x / a.cap);
+            x *= LOG2E;
+            if (mask) {
+                const float add = see ? (float)mask[key] : -INFINITY;
+                see &= add != -INFINITY;
+                x = fmaf(slope, add, x);
+            }
+            s[r] = see ? x : -INFINITY;
+            sees |= see ? 1u << r : 0u;
+            top = fmaxf(top, s[r]);
+        }
+        if (!__any(sees)) continue;
+        top = fmaxf(top, swap32_f(top));
+        const float drop = m == top ? 1.0f : exp2f(m - top), ref = top == -INFINITY ? 0.0f : top;
+        m = top;
+        l *= drop;
+#pragma unroll
+        for (int d = 0; d < NB; ++d) o[d] *= drop;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - ref);
+        // two keys (one of the largest heads) on their way at a time
+        constexpr int AT_ONCE = NB <= 4 ? 2 : 1;
+        typedef TK x4 __attribute__((ext_vector_type(4)));
+        for (int r = 0; r < 16; ++r) {
+#pragma unroll
+            for (int half0 = 0; half0 < 2; half0 += AT_ONCE) {
+                x4 x[AT_ONCE][4 * NB];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const int key = min(j + 8 * (r / 4) + 4 * (half0 + u) + r % 4, j_end - 1);
+                    const TK *vr = reinterpret_cast<const TK *>(vb + key * v_j) + 4 * h;
+#pragma unroll
+                    for (int e = 0; e < 4 * NB; ++e) x[u][e] = 8 * e < a.D ? *reinterpret_cast<const x4 *>(vr + 8 * e) : x4{};
+                }
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const int from = (lane & 31) + 32 * (half0 + u);
+                    const float weight = __shfl(s[0], from, 64);
+                    if (!(__shfl(sees, from, 64) & 1)) continue;
+                    l += weight;
+#pragma unroll
+                    for (int e = 0; e < 16 * NB; ++e) o[e / 16][e % 16] = fmaf(weight, (float)x[u][e / 4][e % 4], o[e / 16][e % 16]);
+                }
+            }
+            // (the next weight and its bit, in the same registers)
+            sees >>= 1;
+#pragma unroll
+            for (int e = 0; e < 15; ++e) s[e] = s[e + 1];
+        }
+        const uint64_t lost = __ballot(l != l);
+        if (((uint32_t)lost & again) == again) break;
+    }
+    if (again >> (lane & 31) & 1) put_row<TQ, NB>(a, p, w, o, m, l);
+}
+
+// a wave's 32 rows, of which this lane's is `row`
+template <typename TK, typename TQ, int DC, bool PREFIX>
+__device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DC / 32], float m, float l, int row0, int row,
                                            bool row_ok, int bh, int split, int j_begin, int j_end) {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    // (a sum of infinities of both signs is NaN too: such a row is done again for nothing, to the same result)
+    const int lane = threadIdx.x & 63;
+    // (a sum of infinities of both signs is NaN too: such a row is formed again for nothing, to the same result)
     float all = l;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
@@ -344,32 +469,9 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
         for (int d = 0; d < DC / 32; ++d) all += o[d][r];
     const bool bad = all != all;
     const uint64_t votes = __ballot(bad && row_ok);
-    uint32_t again = (uint32_t)votes | (uint32_t)(votes >> 32);
-    if (row_ok && !(again >> (lane & 31) & 1)) {
-        const RowOut w = row_out<PREFIX>(a, p, row, bh, split);
-        if (p.part_o && h == 0) {
-            p.part_ml[2 * w.slot] = m;
-            p.part_ml[2 * w.slot + 1] = l;
-        }
-        const float f = p.part_o ? 1.0f : finish(a, w.head, m, l);
-        float *po = p.part_o + w.slot * a.D;
-        TQ *out = reinterpret_cast<TQ *>(a.o + w.i * a.o_i + w.head * a.o_h + w.b * a.o_b);
-#pragma unroll
-        for (int d = 0; d < DC / 32; ++d)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                if (32 * d + 8 * r4 >= a.D) continue;   // (D is a multiple of 8)
-                const int at = 32 * d + 8 * r4 + 4 * h;
-                const f32x4 x = f32x4{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]} * f;
-                if (p.part_o) *reinterpret_cast<f32x4 *>(po + at) = x;
-                else store4<TQ>(out + at, x);
-            }
-    }
-    while (again) {
-        const int at = __builtin_ctz(again);
-        again &= again - 1;
-        redo_row<TK, TQ, PREFIX>(a, p, __builtin_amdgcn_readlane(row, at), bh, split, j_begin, j_end);
-    }
+    const uint32_t again = (uint32_t)votes | (uint32_t)(votes >> 32);
+    if (row_ok && !(again >> (lane & 31) & 1)) put_row<TQ, DC / 32>(a, p, row_out<PREFIX>(a, p, row, bh, split), o, m, l);
+    if (again) redo_rows<TK, TQ, DC, PREFIX>(a, p, row0, again, bh, split, j_begin, j_end);
 }
 
 // the place of piece c (four values) of row r in a wave's stretch of LDS: permuted by the row, against bank conflicts
@@ -377,11 +479,12 @@ template <int DP> __device__ __forceinline__ int piece_at(int r, int c) { return
 
 // up to 32 rows that the waves hold parts of, each in its stretch of LDS (pieces of the rows, then the maxima and
 // the sums): a thread a piece, so that a token's few rows are spread over all threads
-template <typename TK, typename TQ, int DP, int WAVES, bool PREFIX>
+template <typename TK, typename TQ, int DC, int WAVES, bool PREFIX>
 __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p, const char *lds, int stretch, int tops, int row0, int bh,
                                            int split, int j_begin, int j_end) {
-    constexpr int PIECES = DP / 4, AT_ONCE = WAVES * 64 / PIECES;   // of a row; rows
+    constexpr int DP = row_place(DC), PIECES = DP / 4, AT_ONCE = WAVES * 64 / PIECES;   // of a row; rows
     const int lane = threadIdx.x & 63, c = threadIdx.x % PIECES, n = min(32, p.rows - row0);
+    uint32_t bad_rows = 0;
     for (int r0 = 0; r0 < n; r0 += AT_ONCE) {
         const int r = r0 + threadIdx.x / PIECES, row = row0 + min(r, n - 1);
         const bool ok = r < n;
@@ -430,9 +533,10 @@ __device__ __forceinline__ void join_waves(const AttnArgs &a, const AttnPart &p,
         while (again) {
             const int at = __builtin_ctzll(again);
             again &= again - 1;
-            redo_row<TK, TQ, PREFIX>(a, p, __builtin_amdgcn_readlane(row, at), bh, split, j_begin, j_end);
+            bad_rows |= 1u << __builtin_amdgcn_readlane(r, at);
         }
     }
+    if (bad_rows) redo_rows<TK, TQ, DC, PREFIX>(a, p, row0, bad_rows, bh, split, j_begin, j_end);
 }
 
 // the splits' partial results of a row, joined in a fixed order: GROUPS groups of DP / 4 threads a row take
@@ -607,27 +711,21 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 
     float c = a.scale;
     if constexpr (SPLIT) {
-        // (infinities are no measure of the others, and have no second term)
         float top = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(qx[t][e]) < INFINITY ? fabsf(qx[t][e]) : 0.0f);
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, size_of(qx[t][e]));
         top = fmaxf(top, swap32_f(top));
-        // 2^up * q below 2^15: no f16 overflows, and the second term lies as far above f16's subnormals as it can
-        int up = 0;
-        if (top > 0.0f) {
-            (void)frexpf(top, &up);
-            up = 15 - up;
-        }
+        const int up = shift_of(top);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = ldexpf(qx[2 * t + e / 4][e % 4], up);
-                const _Float16 hi = (_Float16)x;
+                _Float16 hi, lo;
+                query_terms(qx[2 * t + e / 4][e % 4], up, hi, lo);
                 qf[t][e] = hi;
-                ql[t][e] = fabsf(x) < INFINITY ? (_Float16)(x - (float)hi) : (_Float16)0.0f;
+                ql[t][e] = lo;
             }
         c = ldexpf(c, -up);
     }
@@ -939,7 +1037,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
             }
         }
         __syncthreads();
-        join_waves<TK, TQ, DP, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
+        join_waves<TK, TQ, DC, WAVES, PREFIX>(a, p, lds, T::STRETCH, 2 * BYTES, row0, bh, split, j_begin, j_end);
     } else {
         if constexpr (TURNS > 1) {
             // the second group leaves its part to the first one, in LDS that no DMA is on its way to: the rows' maxima
@@ -973,7 +1071,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 }
             m = top;
         }
-        store_rows<TK, TQ, DC, PREFIX>(a, p, o, m - BIAS, l, row, row_ok, bh, split, j_begin, j_end);
+        store_rows<TK, TQ, DC, PREFIX>(a, p, o, m - BIAS, l, row0, row, row_ok, bh, split, j_begin, j_end);
     }
 }
 

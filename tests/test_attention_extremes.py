@@ -1,9 +1,14 @@
-"""Attention at the ends of its types' ranges. Allowances are those of tests/test_attention.py, whose `formula` leaves
-out what a row does not see."""
+"""Attention at the ends of its types' ranges: the largest values of a cache, f32 queries whose row holds one value
+far above the others, factors of nothing beside large products, infinities under a cap, and values that are not
+finite in places that some rows see and others do not. Allowances are those of tests/test_attention.py, whose
+`formula` leaves out what a row does not see."""
 import math
 
+import numpy as np
 import pytest
-from test_attention import IDS, INF, PAIRS, TYPES, call, formula, full, near, operands, rnd, torch
+from test_attention import IDS, INF, NAN, PAIRS, TYPES, call, formula, full, near, operands, rnd, torch
+
+import mi355x_qmm as M
 
 gpu = pytest.mark.gpu
 
@@ -116,3 +121,70 @@ def test_next_to_no_factor_beside_large_products(kv, io, n, scale):
     near(call(q, k, v, scale), formula(q, k, v, scale, full(2, 150)))
     near(call(q, k, v, scale, mask=w), formula(q, k, v, scale, full(2, 150), mask=w))
     near(call(q, k, v, scale, kp=kp, vp=vp), formula(q, k, v, scale, full(2, 150), kp=kp, vp=vp))
+
+
+# ---- values that are not finite ----------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("kv,io", PAIRS, ids=IDS)
+@pytest.mark.parametrize("n", [1, 6, 50, 200])
+@pytest.mark.parametrize("D", [40, 64, 96, 128, 184, 256])
+def test_nonfinite_values_that_some_rows_see(kv, io, n, D):
+    """NaN and infinities in single channels of values, in keys that some rows see: those channels of those rows, and
+    nothing else"""
+    m, H = 330, 4
+    q, k, v = operands(1, n, m, H, 2, D, kv, io, seed=n + D)
+    w = rnd((1, H, n, m), "f16", 5)
+    r = torch.from_numpy(np.random.default_rng(6).random((H, n, m)) < 0.4).cuda()
+    w[0][r] = -INF
+    w[..., 7], w[..., 200] = 0.0, -INF
+    marks = [(0, 3, NAN), (7, 1, INF), (31, 5, INF), (32, 5, -INF), (100, D - 1, -INF), (200, 4, NAN), (255, 6, NAN), (256, 7, INF), (329, 3, NAN)]
+    k2, v2 = k.clone(), v.clone()
+    k2[:, 200] = NAN
+    for j, ch, x in marks:
+        v2[0, j, :, ch] = x
+    got = call(q, k2, v2, 0.1, mask=w)[0].double()
+    o, most, _ = formula(q, k, torch.where(torch.isfinite(v2), v2, 0.0), 0.1, full(1, m), mask=w)
+    want = o[0].clone()
+    seen = (w[0] != -INF).permute(1, 0, 2)                     # [n, H, m]
+    for j, ch, x in marks:
+        # (a sum of weights above 0 times these: infinity, or NaN with one of the other sign)
+        want[:, :, ch] = torch.where(seen[:, :, j], want[:, :, ch] + x, want[:, :, ch])
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf])
+    fine = torch.isfinite(want)
+    assert (((got - o[0]).abs() <= most[0]) | ~fine).all(), float(((got - o[0]).abs() - most[0])[fine].max())
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 1000])
+@pytest.mark.parametrize("what", ["hidden value", "hidden key", "seen value"])
+def test_one_nan_costs_no_second(n, what):
+    """the rows whose sums a NaN spoils are formed again, 32 at a time: 1500 keys of up to 1.5 us are 2.3 ms, some 50 of
+    the calls of 45 us; a row at a time takes 2 us for each of its keys, 2000 calls"""
+    m = 1500 if n > 1 else 4000
+    q, k, v = operands(1, n, m, 8, 2, 128, "f16", "f32", seed=1)
+    w = torch.zeros(1, 1, n, m, dtype=torch.float16, device="cuda")
+    if what != "seen value":
+        w[..., 700] = -INF
+    out, spec, hf = torch.empty_like(q), M.attn_spec(0.09), lambda t: M.from_torch(t.permute(0, 2, 1, 3))
+
+    def us():
+        best = INF
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            for _ in range(2):
+                M.flash_attn(hf(q), hf(k), hf(v), M.from_torch(out), spec, mask=M.from_torch(w))
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 500)
+        return best
+
+    before = us()
+    (k if what == "hidden key" else v)[0, 700, 0, 3] = NAN
+    assert us() <= 100 * before
+    assert torch.isnan(out).any() == (what == "seen value")
