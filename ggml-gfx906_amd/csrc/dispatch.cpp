@@ -857,13 +857,13 @@ int ggml_mi355x_flash_attn_prefix(const ggml_mi355x_tensor *q, const ggml_mi355x
     return attn_entry(t, *params, work, work_bytes, stream);
 }
 
-// (the result's and the values' layouts do not matter here: those of q and k stand in)
+// (the result's and the values' layouts do not matter here: a contiguous result and k's stand in)
 static int attn_work_entry(const ggml_mi355x_tensor *q, const ggml_mi355x_tensor *kp, const ggml_mi355x_tensor *k, size_t *bytes) {
     if (!q || !k || !bytes) return GGML_MI355X_EINVAL;
     AttnOptional o;
     AttnTensors t{view_of(q), view_of(k), view_of(k), view_of(q)};
     std::swap(t.dst.ne[1], t.dst.ne[2]);
-    std::swap(t.dst.nb[1], t.dst.nb[2]);
+    for (int i = 1; i < 4; ++i) t.dst.nb[i] = t.dst.nb[i - 1] * (size_t)t.dst.ne[i - 1];
     t.kp = t.vp = o.of(3, kp);
     const ggml_mi355x_attn_params p{1.0f, 0.0f, 0.0f, 0};
     const int rc = check_flash_attn(t, p);

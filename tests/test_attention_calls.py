@@ -1,0 +1,28 @@
+"""Calls of the attention entry points that their documentation allows, and ones that must not reach the GPU. All but
+the last run without a GPU."""
+import pytest
+from test_attention import call, desc, formula, full, near, rnd, torch
+
+import mi355x_qmm as M
+
+gpu = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("nb", [[2, 256, 256, 0], [2, 0, 256, 8192], [2, 256, 0, 256], [2, 0, 0, 0]])
+def test_workspace_of_a_broadcast_query(nb):
+    """one query for several batches, heads or positions: the size is that of queries of their own"""
+    k, kp = desc(M.F16, [128, 9000, 8, 4]), desc(M.F16, [128, 9000, 8])
+    q, own = desc(M.F16, [128, 2, 32, 4], nb), desc(M.F16, [128, 2, 32, 4])
+    assert M.flash_attn_work_size(q, k) == M.flash_attn_work_size(own, k) > 0
+    assert M.flash_attn_prefix_work_size(q, kp, k) == M.flash_attn_prefix_work_size(own, kp, k) > 0
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 40])
+def test_broadcast_query_with_a_workspace(n):
+    q = rnd((1, n, 1, 64), "f16", 1, 1.5).expand(3, n, 8, 64)
+    k, v = rnd((3, 3000, 2, 64), "f16", 2), rnd((3, 3000, 2, 64), "f16", 3)
+    hf = lambda t: M.from_torch(t.permute(0, 2, 1, 3))  # noqa: E731
+    work = torch.empty(max(16, M.flash_attn_work_size(hf(q), hf(k))), dtype=torch.uint8, device="cuda")
+    out = torch.empty(3, n, 8, 64, dtype=torch.float16, device="cuda")
+    near(call(q, k, v, 0.125, work=work, out=out), formula(q, k, v, 0.125, full(3, 3000)))
