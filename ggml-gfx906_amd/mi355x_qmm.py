@@ -166,8 +166,8 @@ _several_gpus = None
 
 
 def _on_current_gpu(*tensors) -> None:
-    """raises for descriptors (from_torch) of tensors on another GPU than the current one: a kernel runs on the
-    current one, and may not reach them"""
+    """raises for descriptors (from_torch) of tensors, and tensors, on another GPU than the current one: a kernel runs
+    on the current one, and may not reach them"""
     global _several_gpus
     if _several_gpus is None:
         import torch
@@ -176,8 +176,10 @@ def _on_current_gpu(*tensors) -> None:
         import torch
         here = torch.cuda.current_device()
         for t in tensors:
-            if getattr(t, "device", here) != here:
-                raise Mi355xError(f"a tensor on GPU {t.device}, the current one is {here}")
+            at = getattr(t, "device", here)
+            at = getattr(at, "index", at)
+            if at != here:
+                raise Mi355xError(f"a tensor on GPU {at}, the current one is {here}")
 
 
 def _stream_ptr(stream) -> int | None:
@@ -233,8 +235,12 @@ def attn_spec(scale: float, max_bias: float = 0.0, logit_softcap: float = 0.0, c
 
 
 def _work(work):
-    """(address, bytes) of a workspace: a torch tensor, or None for the library's own"""
-    return (None, 0) if work is None else (work.data_ptr(), work.numel() * work.element_size())
+    """(address, bytes) of a workspace: a contiguous torch tensor on the GPU, or None for the library's own"""
+    if work is None:
+        return None, 0
+    if not work.is_cuda or not work.is_contiguous():
+        raise Mi355xError(f"a workspace on {work.device}, contiguous: {work.is_contiguous()} (a contiguous tensor on a GPU)")
+    return work.data_ptr(), work.numel() * work.element_size()
 
 
 def flash_attn(q: MmTensor, k: MmTensor, v: MmTensor, dst: MmTensor, spec: AttnSpec, mask: MmTensor = None, sinks: MmTensor = None,
@@ -242,7 +248,7 @@ def flash_attn(q: MmTensor, k: MmTensor, v: MmTensor, dst: MmTensor, spec: AttnS
     """dst [D, H, n_q, B] = softmax(scale q k^T + mask) v (GGML_OP_FLASH_ATTN_EXT); q [D, n_q, H, B],
     k, v [D, n_kv, Hk, Bk]; work: a tensor of flash_attn_work_size bytes"""
     p, n = _work(work)
-    _on_current_gpu(q, k, v, dst, mask, sinks, kv_len)
+    _on_current_gpu(q, k, v, dst, mask, sinks, kv_len, work)
     _check(lib().ggml_mi355x_flash_attn(_ref(q), _ref(k), _ref(v), _ref(mask), _ref(sinks), _ref(kv_len), _ref(dst), _ref(spec),
                                         p, n, _stream_ptr(stream)), "flash_attn")
 
@@ -257,7 +263,7 @@ def flash_attn_prefix(q: MmTensor, kp: MmTensor, vp: MmTensor, k: MmTensor, v: M
                       sinks: MmTensor = None, kv_len: MmTensor = None, work=None, stream=None) -> None:
     """flash_attn of sequences behind a shared prefix kp, vp [D, n_prefix, Hk]; k, v: each one's own cache"""
     p, n = _work(work)
-    _on_current_gpu(q, kp, vp, k, v, dst, sinks, kv_len)
+    _on_current_gpu(q, kp, vp, k, v, dst, sinks, kv_len, work)
     _check(lib().ggml_mi355x_flash_attn_prefix(_ref(q), _ref(kp), _ref(vp), _ref(k), _ref(v), _ref(sinks), _ref(kv_len), _ref(dst),
                                                _ref(spec), p, n, _stream_ptr(stream)), "flash_attn_prefix")
 

@@ -1,7 +1,8 @@
-"""Calls of the attention entry points that their documentation allows, and ones that must not reach the GPU. All but
-the last run without a GPU."""
+"""Calls of the attention entry points that their documentation allows, and ones that must not reach the GPU."""
+import types
+
 import pytest
-from test_attention import call, desc, formula, full, near, rnd, torch
+from test_attention import base, call, desc, formula, full, near, rnd, torch
 
 import mi355x_qmm as M
 
@@ -26,3 +27,30 @@ def test_broadcast_query_with_a_workspace(n):
     work = torch.empty(max(16, M.flash_attn_work_size(hf(q), hf(k))), dtype=torch.uint8, device="cuda")
     out = torch.empty(3, n, 8, 64, dtype=torch.float16, device="cuda")
     near(call(q, k, v, 0.125, work=work, out=out), formula(q, k, v, 0.125, full(3, 3000)))
+
+
+def tensor_at(index, contiguous=True, kind="cuda"):
+    """what the checks look at of a workspace tensor"""
+    return types.SimpleNamespace(device=torch.device(kind, index), is_cuda=kind == "cuda", is_contiguous=lambda: contiguous, data_ptr=lambda: 0x10000,
+                                 numel=lambda: 1 << 20, element_size=lambda: 1)
+
+
+@pytest.mark.parametrize("work", [torch.empty(1 << 20, dtype=torch.uint8), torch.empty(16, dtype=torch.uint8).expand(1 << 16, 16), tensor_at(0, False)],
+                         ids=["host", "host broadcast", "strided"])
+def test_workspaces_that_a_kernel_may_not_write(work):
+    """host memory would be written by the GPU, a broadcast one behind its end"""
+    a = base()
+    with pytest.raises(M.Mi355xError, match="workspace"):
+        M.flash_attn(a["q"], a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
+    with pytest.raises(M.Mi355xError, match="workspace"):
+        M.flash_attn_prefix(a["q"], desc(M.F16, [64, 70, 2]), desc(M.F16, [64, 70, 2]), a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
+
+
+def test_workspaces_on_another_gpu_are_refused(monkeypatch):
+    monkeypatch.setattr(M, "_several_gpus", True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    a, work = base(), tensor_at(1)
+    with pytest.raises(M.Mi355xError, match="GPU 1"):
+        M.flash_attn(a["q"], a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
+    with pytest.raises(M.Mi355xError, match="GPU 1"):
+        M.flash_attn_prefix(a["q"], desc(M.F16, [64, 70, 2]), desc(M.F16, [64, 70, 2]), a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
