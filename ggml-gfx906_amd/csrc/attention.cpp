@@ -47,12 +47,14 @@ static int check_attn(const AttnTensors &t, const AttnSpec &p) {
     if (D < 8 || D > ATTN_MAX_D || D % 8 != 0 || k.ne[0] != D || v.ne[0] != D) return GGML_MI355X_EINVAL;
     for (int i = 1; i < 4; ++i)
         if (k.ne[i] != v.ne[i]) return GGML_MI355X_EINVAL;
-    if (k.ne[2] <= 0 || H % k.ne[2] != 0 || k.ne[3] <= 0 || B % k.ne[3] != 0) return GGML_MI355X_EINVAL;
+    // (no heads or no batches have a cache of none)
+    auto shared = [](int64_t n, int64_t by) { return by > 0 ? n % by == 0 : n == 0 && by == 0; };
+    if (!shared(H, k.ne[2]) || !shared(B, k.ne[3])) return GGML_MI355X_EINVAL;
     // (a grid has less than 2^32 threads: 256 for every row's join or problem, 512 for 256 rows of a prompt)
     if (H > 65535 || B > 65535 || n_q >= (1 << 24) || H * B > (1 << 22) || H * B * n_q > (t.kp ? 1 << 25 : 1 << 28)) return GGML_MI355X_EINVAL;
     if (d.ne[0] != D || d.ne[1] != H || d.ne[2] != n_q || d.ne[3] != B) return GGML_MI355X_EINVAL;
     for (int i = 1; i < 4; ++i)
-        if (d.ne[i] > 1 && d.nb[i] == 0) return GGML_MI355X_EINVAL;   // two rows in one place
+        if (d.ne[i] > 1 && d.nb[i] == 0 && H * B * n_q > 0) return GGML_MI355X_EINVAL;   // two rows in one place
     if (t.kp) {
         const TensorView &kp = *t.kp, &vp = *t.vp;
         if (kp.type != k.type || vp.type != k.type || t.mask) return GGML_MI355X_EINVAL;
@@ -64,7 +66,7 @@ static int check_attn(const AttnTensors &t, const AttnSpec &p) {
     if (t.mask) {
         const TensorView &m = *t.mask;
         if (m.type != T_F16 || !dims_fit(m) || m.nb[0] != 2 || !aligned_to(m, 2) || m.ne[0] < k.ne[1] || m.ne[1] < n_q) return GGML_MI355X_EINVAL;
-        if (m.ne[2] <= 0 || m.ne[3] <= 0 || H % m.ne[2] != 0 || B % m.ne[3] != 0) return GGML_MI355X_EINVAL;
+        if (!shared(H, m.ne[2]) || !shared(B, m.ne[3])) return GGML_MI355X_EINVAL;
     }
     if (t.sinks && (t.sinks->type != T_F32 || t.sinks->ne[0] < H || t.sinks->nb[0] != 4 || (uintptr_t)t.sinks->data % 4 != 0)) return GGML_MI355X_EINVAL;
     if (t.len) {
@@ -193,6 +195,7 @@ static AttnPlan plan_attn(const AttnTensors &t) {
 }
 
 size_t flash_attn_work(const AttnTensors &t) {
+    if (t.q.ne[1] == 0 || t.q.ne[2] == 0 || t.q.ne[3] == 0) return 0;
     const AttnPlan p = plan_attn(t);
     return p.slots > 1 ? (size_t)t.q.ne[1] * t.q.ne[2] * t.q.ne[3] * p.slots * (t.q.ne[0] + 2) * sizeof(float) : 0;
 }

@@ -2,7 +2,7 @@
 import types
 
 import pytest
-from test_attention import base, call, desc, formula, full, near, rnd, torch
+from test_attention import base, call, desc, formula, full, near, rc, rnd, torch
 
 import mi355x_qmm as M
 
@@ -54,3 +54,28 @@ def test_workspaces_on_another_gpu_are_refused(monkeypatch):
         M.flash_attn(a["q"], a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
     with pytest.raises(M.Mi355xError, match="GPU 1"):
         M.flash_attn_prefix(a["q"], desc(M.F16, [64, 70, 2]), desc(M.F16, [64, 70, 2]), a["k"], a["v"], a["dst"], a["params"], work=work, stream=0)
+
+
+@pytest.mark.parametrize("B,n,H,Hk,Bk", [(0, 3, 8, 2, 0), (0, 3, 8, 2, 1), (2, 3, 0, 0, 2), (2, 3, 0, 2, 2), (2, 0, 8, 2, 2), (0, 0, 0, 0, 0)])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_calls_without_rows(prefix, B, n, H, Hk, Bk):
+    """no sequences, no queries or no heads, beside a cache of none: nothing to do, and no workspace"""
+    cache = desc(M.F16, [64, 50, Hk, Bk])
+    q, kp = desc(M.F16, [64, n, H, B]), desc(M.F16, [64, 70, Hk])
+    more = dict(kp=kp, vp=kp) if prefix else {}
+    want = -1 if prefix and Bk != B else 0   # (behind a prefix every sequence has its own cache)
+    assert rc(prefix, q=q, k=cache, v=cache, dst=desc(M.F16, [64, H, n, B]), **more) == want
+    if not prefix:
+        assert rc(q=q, k=cache, v=cache, dst=desc(M.F16, [64, H, n, B]), mask=desc(M.F16, [50, 3, H, B])) == 0
+        assert rc(q=q, k=cache, v=cache, dst=desc(M.F16, [64, H, n, B]), mask=desc(M.F16, [50, 3])) == 0
+    if want == 0:
+        assert (M.flash_attn_prefix_work_size(q, kp, cache) if prefix else M.flash_attn_work_size(q, cache)) == 0
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+def test_rows_without_a_cache_are_refused(prefix):
+    assert prefix or rc(mask=desc(M.F16, [50, 3, 0, 1])) == rc(mask=desc(M.F16, [50, 3, 1, 0])) == -1
+    for Hk, Bk in ((0, 2), (2, 0), (0, 0)):
+        cache = desc(M.F16, [64, 50, Hk, Bk])
+        more = dict(kp=desc(M.F16, [64, 70, Hk]), vp=desc(M.F16, [64, 70, Hk])) if prefix else {}
+        assert rc(prefix, k=cache, v=cache, **more) == -1
