@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // so that small ones stay clear of its subnormals (f16 values times them stay far below f32's end); bf16 ones
 // up to 1, since a bf16 value may lie anywhere in f32's range and its product must too.
 // F32 queries: q (scaled by a power of two per row) and p are each carried as a sum of two f16 values, two MFMAs per
-// product: to 2^-22 of the value, or of q 2^-40 of its row's largest, of p 2^-33 of the largest weight.
+// product: to 2^-22 of the value, or of q 2^-40 of its row's largest, of p 2^-33 of the largest weight. 16-bit ones: p
+// so too where keys are split (bf16: to 2^-16), else rounded to their type; its sum is of the unrounded weights.
 //
 // Bound by the matrix cores and, beside them, the vector units' exponentials, maxima and sums where a key
 // meets many rows: 8192 causal tokens, 32 heads on 8 of 128 bf16 values 528 us, 1.04 PFLOP/s (a large library product
@@ -918,6 +919,13 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     };
     // (-1 that the compiler does not see: a second term is then one mixed fma, not a conversion, a difference and
     // another conversion)
+    // Weights of 16-bit activations are two terms as well where the waves split the keys: bound by memory, the second
+    // product costs next to nothing (64 x 8192 f16 keys of 8 heads of 128 values 303 and 302 us, of 64 values 201 and
+    // 203), and the result is off by its own rounding alone, rms 2.1e-4 of it, with rounded weights 2.9e-4 (bf16 1.6e-3,
+    // 2.3e-3). Row tiles round them: two terms take 8192 causal
+    // tokens from 513 to 681 us, 64 sequences behind 8192 shared keys from 36 to 39.
+    constexpr bool TWO = SPLIT || !BY_ROWS;
+    constexpr int PV = TWO ? 2 : 1;
     float minus = -1.0f;
     asm("" : "+s"(minus));
     auto values = [&](const char *vt) {
@@ -934,7 +942,7 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 const x2 hi = __builtin_convertvector(x, x2);
                 pf[e] = hi[0];
                 pf[e + 1] = hi[1];
-                if constexpr (SPLIT) {
+                if constexpr (TWO) {
                     pl[e] = (TK)fmaf(minus, (float)hi[0], x[0]);
                     pl[e + 1] = (TK)fmaf(minus, (float)hi[1], x[1]);
                 }
@@ -947,16 +955,16 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
                 const i16x8 vv = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
                 const x8 vf = __builtin_bit_cast(x8, vv);
                 o[d] = mma(vf, pf, o[d]);
-                if constexpr (SPLIT) o[d] = mma(vf, pl, o[d]);
+                if constexpr (TWO) o[d] = mma(vf, pl, o[d]);
             }
         }
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 1);
 #pragma unroll
         for (int n = AHEAD; n < KT / 16 * NB; ++n) {
-            __builtin_amdgcn_sched_group_barrier(0x008, PER, 1);
+            __builtin_amdgcn_sched_group_barrier(0x008, PV, 1);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, PER * AHEAD, 1);
+        __builtin_amdgcn_sched_group_barrier(0x008, PV * AHEAD, 1);
     };
 
     if constexpr (BY_ROWS) {

@@ -178,8 +178,9 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
  * (with a mask as well: both hold). Keys that a row does not see take no part in it, whatever their
  * bytes hold; rows that see no key are zeros. logit_softcap c > 0: scaled scores become
  * c tanh(score / c) before the mask. F32 queries and their weights are each taken as a sum of two F16 terms, exact
- * to 2^-22 of the value (or 2^-40 of the row's largest query value, 2^-33 of its largest weight); with F16 / BF16
- * queries the weights are rounded to that type for the product with v. Results do not depend on
+ * to 2^-22 of the value (or 2^-40 of the row's largest query value, 2^-33 of its largest weight). With F16 / BF16
+ * queries the weights are a sum of two terms of that type where at most 32 rows share a key head (n_q * H / Hk; of a
+ * shared prefix all sequences' rows count), and beyond that rounded to it for the product with v. Results do not depend on
  * timing: every sum has a fixed order.
  *
  * D: a multiple of 8, at most 256. H, B: at most 65535, H B 2^22; n_q: below 2^24; H B n_q: at most 2^28.

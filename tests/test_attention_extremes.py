@@ -188,3 +188,26 @@ def test_one_nan_costs_no_second(n, what):
     (k if what == "hidden key" else v)[0, 700, 0, 3] = NAN
     assert us() <= 100 * before
     assert torch.isnan(out).any() == (what == "seen value")
+
+
+# ---- weights of 16-bit activations -------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("io", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [(3, 1, 1000, 8, 2, 128, 0), (1, 4, 700, 32, 4, 64, 0), (2, 2, 300, 14, 2, 96, 0), (1, 1, 5000, 16, 1, 256, 0), (2, 3, 90, 6, 2, 184, 0),
+                                  (1, 8, 400, 8, 2, 128, 500), (4, 1, 200, 8, 1, 64, 900)], ids=lambda s: "x".join(map(str, s)))
+def test_few_rows_keep_their_weights(io, size):
+    """up to 32 rows a key head: nothing is rounded to 16 bits but the result. Weights of two terms are off by 2^-16 of
+    them (bf16) or 2^-22 and, below f16's normal numbers, 2^-33 of the largest"""
+    B, n, m, H, Hk, D, P = size
+    q, k, v = operands(B, n, m, H, Hk, D, io, io, seed=sum(size))
+    more = dict(kp=rnd((P, Hk, D), io, 7), vp=rnd((P, Hk, D), io, 8)) if P else {}
+    s = 1 / math.sqrt(D)
+    got = call(q, k, v, s, causal=True, **more).double()
+    o, most, _ = formula(q.float(), k, v, s, full(B, m), causal=True, **more)
+    size_of = {name: t.abs() for name, t in more.items() if name == "vp"}
+    A, _, _ = formula(q.float(), k, v.abs(), s, full(B, m), causal=True, **{**more, **size_of})
+    eps = torch.finfo(TYPES[io]).eps / 2
+    weights = 2.0**-16 * A if io == "bf16" else 2.0**-22 * A + 2.0**-33 * (m + P) * float(v.abs().max())
+    assert ((got - o).abs() <= most + weights + eps * o.abs() + torch.finfo(TYPES[io]).tiny * eps).all()
