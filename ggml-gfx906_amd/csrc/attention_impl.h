@@ -716,18 +716,31 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, size_of(qx[t][e]));
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(qx[t][e]));
+        const bool infinite = __any(top == INFINITY);   // (hardly ever)
+        if (infinite) {
+            top = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, size_of(qx[t][e]));
+        }
         top = fmaxf(top, swap32_f(top));
         const int up = shift_of(top);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                _Float16 hi, lo;
-                query_terms(qx[2 * t + e / 4][e % 4], up, hi, lo);
-                qf[t][e] = hi;
-                ql[t][e] = lo;
+                const float x = ldexpf(qx[2 * t + e / 4][e % 4], up);
+                qf[t][e] = (_Float16)x;
+                ql[t][e] = (_Float16)(x - (float)qf[t][e]);
             }
+        if (infinite) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ql[t][e] = fabsf((float)qf[t][e]) < INFINITY ? ql[t][e] : (_Float16)0.0f;
+        }
         c = ldexpf(c, -up);
     }
     const bool capped = KIND != OWN && a.cap != 0.0f;
