@@ -461,7 +461,6 @@ __device__ __forceinline__ void redo_rows(const AttnArgs &a, const AttnPart &p, 
 template <typename TK, typename TQ, int DC, bool PREFIX>
 __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p, const f32x16 (&o)[DC / 32], float m, float l, int row0, int row,
                                            bool row_ok, int bh, int split, int j_begin, int j_end) {
-    const int lane = threadIdx.x & 63;
     // (a sum of infinities of both signs is NaN too: such a row is formed again for nothing, to the same result)
     float all = l;
 #pragma unroll
@@ -471,7 +470,9 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const AttnPart &p,
     const bool bad = all != all;
     const uint64_t votes = __ballot(bad && row_ok);
     const uint32_t again = (uint32_t)votes | (uint32_t)(votes >> 32);
-    if (row_ok && !(again >> (lane & 31) & 1)) put_row<TQ, DC / 32>(a, p, row_out<PREFIX>(a, p, row, bh, split), o, m, l);
+    // (such rows too, under their new values: registers enough for a branch less, 2000 masked queries of 64-value heads 90.9 us
+    // and 88.0)
+    if (row_ok) put_row<TQ, DC / 32>(a, p, row_out<PREFIX>(a, p, row, bh, split), o, m, l);
     if (again) redo_rows<TK, TQ, DC, PREFIX>(a, p, row0, again, bh, split, j_begin, j_end);
 }
 
