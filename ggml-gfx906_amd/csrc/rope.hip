@@ -7,9 +7,9 @@
 // n_dims are copied. The gradient turns by -t: a turn's transpose is its inverse, and `size` stays.
 //
 // Angles are formed in 64 bits as turns: pos * f_i / 2pi less its nearest whole number, and only
-// that remainder (|.| <= 1/2) is rounded to 32 bits: 2^-26 of a turn, beside two roundings of the
-// 64-bit product (2^-52 of the turns made: 2^-25 at position 2^31). A 32-bit angle of 1e6 radians
-// would be off by up to 0.03.
+// that remainder (|.| <= 1/2) is rounded to 32 bits: 2^-26 of a turn, beside the roundings of the
+// 64-bit frequency and product (2^-53 each of the turns made, together 2^-23.6 of a turn at position
+// 2^31; a third one where a factor divides). A 32-bit angle of 1e6 radians would be off by up to 0.03.
 #include "../../include/ggml-mi355x.h"
 #include "dispatch.h"
 #include "qcommon.h"

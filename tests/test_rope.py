@@ -130,6 +130,19 @@ def test_far_and_negative_positions():
 
 
 @gpu
+@pytest.mark.parametrize("factors", [False, True])
+def test_far_positions_to_their_roundings(factors):
+    """the frequency and its product with the position are off by 2^-53 each of the radians made, a division by factors by
+    as much again"""
+    pos = np.array([[2**31 - 1 - 97 * i for i in range(20)] + [-(2**31) + 89 * i for i in range(20)]], dtype=np.int32)
+    x = values((1, 40, 2, 128), "f32", 5)
+    ff = (1 + 7 * np.random.default_rng(1).random(64)).astype(np.float32) if factors else None
+    for mode in (M.ROPE_NEIGHBOURS, M.ROPE_HALVES):
+        spec = M.rope_spec(128, mode)
+        near(run(x, pos[0], spec, factors=ff), *turned(x.double().cpu().numpy(), pos, spec, ff), "f32", extra=(3 if factors else 2) * 2.0**-53 * 2.0**31)
+
+
+@gpu
 @pytest.mark.parametrize("mode", [M.ROPE_NEIGHBOURS, M.ROPE_HALVES])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_in_place_strides_and_what_lies_between(mode, dtype):
