@@ -161,11 +161,11 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const AttnArgs a) {
 // so too where keys are split (bf16: to 2^-16), else rounded to their type; its sum is of the unrounded weights.
 //
 // Bound by the matrix cores and, beside them, the vector units' exponentials, maxima and sums where a key
-// meets many rows: 8192 causal tokens, 32 heads on 8 of 128 bf16 values 528 us, 1.04 PFLOP/s (a large library product
-// reaches 1.2). By memory where it meets few: 64 tokens, the same heads in f16, ragged to 8192 keys 295 us,
+// meets many rows: 8192 causal tokens, 32 heads on 8 of 128 bf16 values 531 us, 1.04 PFLOP/s (a large library product
+// reaches 1.2). By memory where it meets few: 64 tokens, the same heads in f16, ragged to 8192 keys 291 us,
 // 5.5 TB/s; one token behind 131072 keys 101 us, 5.3. By latency in small calls: one token's 12 heads of 64
-// values, 1000 keys 6.3 us and 3.4 for the join. A mask's rows lie across a load's lanes: 16 heads of 80 values,
-// 2 x 777 queries, 1900 keys, f32, 59 us, 46 without a mask.
+// values, 1000 keys 6.0 us and 3.3 for the join. A mask's rows lie across a load's lanes: 16 heads of 80 values,
+// 2 x 777 queries, 1900 keys, f32, 58 us, 46 without a mask.
 // ------------------------------------------------------------------------------------------
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

@@ -191,7 +191,8 @@ GGML_MI355X_API int ggml_mi355x_rope_back(const ggml_mi355x_tensor *src, const g
  * work: a workspace of ggml_mi355x_flash_attn_work_size() bytes (16-byte aligned), used only until the
  * call's kernels are done, or NULL: the library keeps one per (device, stream), which can not grow inside
  * a stream capture (ENOMEM: run the call once before capturing it) and which captured graphs of one
- * stream share: graphs that may run at the same time need workspaces of their own. A graph keeps the
+ * stream share with each other and with that stream's own calls: those that may run at the same time need
+ * workspaces of their own. A graph keeps the
  * workspace it was captured with when a later call needs a larger one. */
 typedef struct {
     float   scale, max_bias, logit_softcap;
