@@ -440,10 +440,12 @@ __device__ __forceinline__ void redo_rows(const AttnArgs &a, const AttnPart &p, 
                 for (int u = 0; u < AT_ONCE; ++u) {
                     const int from = (lane & 31) + 32 * (half0 + u);
                     const float weight = __shfl(s[0], from, 64);
-                    if (!(__shfl(sees, from, 64) & 1)) continue;
-                    l += weight;
+                    const bool see = __shfl(sees, from, 64) & 1;
+                    if (see) {
+                        l += weight;
 #pragma unroll
-                    for (int e = 0; e < 16 * NB; ++e) o[e / 16][e % 16] = fmaf(weight, (float)x[u][e / 4][e % 4], o[e / 16][e % 16]);
+                        for (int e = 0; e < 16 * NB; ++e) o[e / 16][e % 16] = fmaf(weight, (float)x[u][e / 4][e % 4], o[e / 16][e % 16]);
+                    }
                 }
             }
             // (the next weight and its bit, in the same registers)
@@ -936,8 +938,8 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs &a, const AttnPart &p,
     // Weights of 16-bit activations are two terms as well where the waves split the keys: bound by memory, the second
     // product costs next to nothing (64 x 8192 f16 keys of 8 heads of 128 values 303 and 302 us, of 64 values 201 and
     // 203), and the result is off by its own rounding alone, rms 2.1e-4 of it, with rounded weights 2.9e-4 (bf16 1.6e-3,
-    // 2.3e-3). Row tiles round them: two terms take 8192 causal
-    // tokens from 513 to 681 us, 64 sequences behind 8192 shared keys from 36 to 39.
+    // 2.3e-3). Row tiles round them: two terms take 8192 causal tokens from 513 to 681 us, 64 sequences behind 8192
+    // shared keys from 36 to 39.
     constexpr bool TWO = SPLIT || !BY_ROWS;
     constexpr int PV = TWO ? 2 : 1;
     float minus = -1.0f;
